@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define P3D_ABI_VERSION 23
+#define P3D_ABI_VERSION 24
 
 enum p3d_status { P3D_OK = 0, P3D_EINVAL = 1, P3D_EHIP = 2, P3D_EUNSUPPORTED = 3 };
 enum p3d_dtype { P3D_F32 = 0, P3D_F16 = 1, P3D_BF16 = 2 };
@@ -552,6 +552,115 @@ int p3d_cast(const p3d_cast_job* jobs, int32_t count, void* stream);
  * the columns past the last row: the weights operand of p3d_input_grad. */
 int p3d_concat_transpose(const void* w0, int32_t out0, const void* w1, int32_t out1, const void* w2, int32_t out2,
                          int32_t dim, void* wt, int32_t k_pad, void* stream);
+
+/* ---- around the block (no counterpart in the reference) ----------------- */
+
+/* A dropout mask: element i of a tensor in row-major order is dropped where 16
+ * bits, half i % 8 (low halves first) of Philox4x32-10 for the counter
+ * (i / 8, offset) and the key seed, are below `threshold` (0 to 65535; 0 drops
+ * nothing); what is kept is divided by 1 - threshold / 65536.  state (device
+ * memory, or NULL): seed and offset as two int64, read by the kernel in place of
+ * the two fields. */
+typedef struct p3d_dropout {
+    const int64_t* state;
+    int64_t seed, offset;
+    int32_t threshold, pad_;
+} p3d_dropout;
+
+/* y = dropout(x) for contiguous x and y of `count` elements of dtype. */
+int p3d_dropout_apply(const void* x, void* y, int64_t count, int32_t dtype, const p3d_dropout* dropout, void* stream);
+
+enum p3d_norm_kind { P3D_NORM_NONE = 0, P3D_NORM_LAYER = 1, P3D_NORM_RMS = 2 };
+enum p3d_gate_kind { P3D_GATE_NONE = 0, P3D_GATE_SAMPLE = 1, P3D_GATE_TOKEN = 2, P3D_GATE_FULL = 3 };
+
+/* (x - mean) / sqrt(var + eps) * weight + bias (layer) or x / sqrt(mean(x^2) + eps)
+ * * weight + bias (rms); weight and bias [dim] or NULL. */
+typedef struct p3d_norm {
+    const void* weight;
+    const void* bias;
+    int32_t kind; /* enum p3d_norm_kind */
+    float eps;
+} p3d_norm;
+
+/* The end of a block over samples * tokens rows of dim channels (1 to 8192):
+ *   out = alpha x + scale * gate * dropout(post(y)),   n = next(out),
+ * or, without y, the norm before a block, n = next(x).  x, out, dout and dx have
+ * type `outer`, y, n, dn and dy type `inner` (outer fp32, or both the same); the
+ * parameters (norm weights and biases, scale [dim] or NULL) type `param`.  Rows
+ * have unit channel stride and the given strides (in elements, any alignment);
+ * outputs are contiguous.  gate: one row of dim channels a sample, one value a
+ * token, or one an element, gate_stride elements apart.  The dropout mask indexes
+ * y as [rows, dim].
+ *
+ * Forward: writes out (with y), n (with next) and, if stats is not NULL, the
+ * statistics that the backward reads: fp32 [4][rows], mean and 1 / sqrt of y (post),
+ * then of out (next).
+ *
+ * Backward (p3d_block_bwd), with the forward's arguments and dout and / or dn: dx,
+ * dy and dgate (per token or element, of gate_dtype, contiguous) where they are
+ * not NULL; for a gate per sample dgate_part, fp32 [splits][samples][dim], to be
+ * summed over the splits; and part, fp32 [grid][5][dim], to be summed over the
+ * grid: the gradients of post weight and bias, scale, next weight and bias (rows of
+ * parameters that are NULL, and of next without dn, are left as they were).
+ *
+ * splits: ranges that a sample's rows are cut into, at most `tokens`; grid:
+ * workgroups, at most splits * samples. */
+typedef struct p3d_block_args {
+    int64_t tokens;
+    int32_t samples, splits, grid, dim;
+    int32_t outer, inner, param, gate_dtype, gate_kind; /* gate_kind: enum p3d_gate_kind */
+    float alpha;
+    const void* x;
+    const void* y;
+    int64_t x_stride, y_stride;
+    const void* gate;
+    int64_t gate_stride;
+    const void* scale;
+    p3d_norm post, next;
+    p3d_dropout dropout;
+    void* out;
+    void* n;
+    float* stats;
+    const void* dout;
+    const void* dn;
+    int64_t dout_stride, dn_stride;
+    void* dx;
+    void* dy;
+    void* dgate;
+    float* dgate_part;
+    float* part;
+} p3d_block_args;
+
+int p3d_block_fwd(const p3d_block_args* args, void* stream);
+int p3d_block_bwd(const p3d_block_args* args, void* stream);
+
+/* Rotary positions of `count` (1 to 4) tensors x[k] [batch, heads[k], tokens,
+ * head_dim] into y[k], views with unit channel stride at any element alignment.
+ * Pair j < pairs (2 pairs <= head_dim) turns by positions[axis] * freqs[j] radians and is multiplied by
+ * magnitude: channels 2j, 2j + 1, or j, pairs + j with half != 0; the channels from
+ * 2 pairs on are copied.  The first axis_pairs[0] pairs are on axis 0, the next
+ * axis_pairs[1] on axis 1, the rest on axis 2.  positions: int32 (or int64, with
+ * pos_is64), strides in elements per batch entry (0: shared), token and axis.
+ * inverse != 0 turns back (the gradient).  heads[k] * ceil(head_dim / 8) must be at
+ * most about 8192. */
+typedef struct p3d_rotary_args {
+    p3d_view x[4], y[4];
+    int32_t heads[4];
+    int64_t tokens;
+    int32_t count, batch, head_dim, pairs, axes;
+    int32_t axis_pairs[3];
+    const void* positions;
+    int64_t pos_sb, pos_sn, pos_sa;
+    const double* freqs; /* [pairs], radians a position */
+    int32_t pos_is64, half, inverse, dtype;
+    float magnitude;
+    int32_t pad_;
+} p3d_rotary_args;
+
+int p3d_rotary(const p3d_rotary_args* args, void* stream);
+
+/* sizeof of p3d_dropout, p3d_norm, p3d_block_args, p3d_rotary_args into out[4]. */
+int p3d_block_struct_sizes(int64_t* out);
 
 /* ---- self-tests (no counterpart in the reference) ---------------------- */
 

@@ -25,7 +25,7 @@ class View(ctypes.Structure):
     _fields_ = [("data", c_void_p), ("sb", c_int64), ("sh", c_int64), ("sn", c_int64)]
 
 
-ABI_VERSION = 23  # P3D_ABI_VERSION in include/pack3d_hip.h
+ABI_VERSION = 24  # P3D_ABI_VERSION in include/pack3d_hip.h
 
 
 class Rope(ctypes.Structure):
@@ -87,6 +87,33 @@ class CastJob(ctypes.Structure):
                 ("dst_dtype", c_int32)]
 
 
+class Dropout(ctypes.Structure):
+    _fields_ = [("state", c_void_p), ("seed", c_int64), ("offset", c_int64), ("threshold", c_int32), ("pad_", c_int32)]
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = [("weight", c_void_p), ("bias", c_void_p), ("kind", c_int32), ("eps", c_float)]
+
+
+class BlockArgs(ctypes.Structure):
+    _fields_ = [("tokens", c_int64), ("samples", c_int32), ("splits", c_int32), ("grid", c_int32), ("dim", c_int32),
+                ("outer", c_int32), ("inner", c_int32), ("param", c_int32), ("gate_dtype", c_int32),
+                ("gate_kind", c_int32), ("alpha", c_float), ("x", c_void_p), ("y", c_void_p), ("x_stride", c_int64),
+                ("y_stride", c_int64), ("gate", c_void_p), ("gate_stride", c_int64), ("scale", c_void_p),
+                ("post", NormArgs), ("next", NormArgs), ("dropout", Dropout), ("out", c_void_p), ("n", c_void_p),
+                ("stats", c_void_p), ("dout", c_void_p), ("dn", c_void_p), ("dout_stride", c_int64),
+                ("dn_stride", c_int64), ("dx", c_void_p), ("dy", c_void_p), ("dgate", c_void_p),
+                ("dgate_part", c_void_p), ("part", c_void_p)]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [("x", View * 4), ("y", View * 4), ("heads", c_int32 * 4), ("tokens", c_int64), ("count", c_int32),
+                ("batch", c_int32), ("head_dim", c_int32), ("pairs", c_int32), ("axes", c_int32),
+                ("axis_pairs", c_int32 * 3), ("positions", c_void_p), ("pos_sb", c_int64), ("pos_sn", c_int64),
+                ("pos_sa", c_int64), ("freqs", c_void_p), ("pos_is64", c_int32), ("half", c_int32),
+                ("inverse", c_int32), ("dtype", c_int32), ("magnitude", c_float), ("pad_", c_int32)]
+
+
 _P = c_void_p
 SIGNATURES = {
     "p3d_last_error": ([], ctypes.c_char_p),
@@ -140,6 +167,11 @@ SIGNATURES = {
     "p3d_gate_fwd": ([_P, c_int32, _P, c_int32, c_int64, _P], c_int32),
     "p3d_gate_bwd": ([_P, c_int32, View, c_int32, _P, _P, c_int32, c_int32, c_int64, _P], c_int32),
     "p3d_cast": ([ctypes.POINTER(CastJob), c_int32, _P], c_int32),
+    "p3d_dropout_apply": ([_P, _P, c_int64, c_int32, ctypes.POINTER(Dropout), _P], c_int32),
+    "p3d_block_fwd": ([ctypes.POINTER(BlockArgs), _P], c_int32),
+    "p3d_block_bwd": ([ctypes.POINTER(BlockArgs), _P], c_int32),
+    "p3d_rotary": ([ctypes.POINTER(RotaryArgs), _P], c_int32),
+    "p3d_block_struct_sizes": ([_P], c_int32),
     "p3d_concat_transpose": ([_P, c_int32, _P, c_int32, _P, c_int32, c_int32, _P, c_int32, _P], c_int32),
 }
 
@@ -262,6 +294,16 @@ def sum_rows(jobs, device):
     args = (SumJob * len(jobs))(*[SumJob(src[0], out.data_ptr(), src[1], src[2], out.numel(), DTYPES[out.dtype])
                                   for src, (_, out) in zip(srcs, jobs)])
     call("p3d_sum_rows", args, len(jobs), stream_of(device))
+
+
+def launch(name, device, *args):
+    """``call`` on the device's current stream, with that device current (a
+    launch goes to the current device, whatever stream it is given)."""
+    if torch.cuda.current_device() == device.index:
+        call(name, *args, stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream_of(device))
 
 
 def require_device(t: torch.Tensor, what="tensor"):

@@ -32,7 +32,7 @@ FLAGS = ["-x", "hip", "-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-fno-honor-nans", "-Wno-nan-infinity-disabled"]
 # Sources whose outputs a loss scaler looks at for what overflowed.
-HONOR_NANS = ("params.hip",)
+HONOR_NANS = ("params.hip", "block_fwd.hip", "block_bwd.hip", "dropout.hip", "rotary.hip")
 
 
 def _hipcc():

@@ -56,3 +56,12 @@ extern "C" int p3d_struct_sizes(int64_t* out) {
     out[5] = sizeof(p3d_project_args);
     return P3D_OK;
 }
+
+extern "C" int p3d_block_struct_sizes(int64_t* out) {
+    P3D_REQUIRE(out, "null argument");
+    out[0] = sizeof(p3d_dropout);
+    out[1] = sizeof(p3d_norm);
+    out[2] = sizeof(p3d_block_args);
+    out[3] = sizeof(p3d_rotary_args);
+    return P3D_OK;
+}

@@ -1,0 +1,197 @@
+"""Rotary positions of queries and keys: interleaved or half layout, whole heads or
+part of them, one to three axes of coordinates, frequencies scaled for grids and
+sequences beyond those of training.
+
+``apply_rotary`` turns up to four tensors in one launch (``p3d_rotary``): before
+``pack3d_hip``, which takes rotated q, kl and kg, or anywhere else.  The layer's
+own rotation (``rope.py``) is fused into its kernels, for whole interleaved heads
+and frequencies as trained.  ``rotary_frequencies`` makes the frequencies;
+``RotaryEncoding`` holds a choice of all this for ``PACK3DAttention``.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .rope import _cached
+
+LAYOUTS = ("interleaved", "half")
+SCALINGS = ("none", "linear", "ntk", "parts")
+MAX_TENSORS = 4
+
+
+def rotary_frequencies(pairs, *, base=10000.0, scaling="none", factor=1.0, trained=None, fast=32.0, slow=1.0):
+    """(frequencies, magnitude): radians a position of each pair, float64 [sum(pairs)]
+    on the CPU, for the pair counts of one to three axes (an int: one axis).
+
+    Pair j of an axis of c pairs turns by base^(-j / c).  For positions up to
+    ``factor`` times those of training: "linear" divides every frequency by factor
+    (positions interpolated); "ntk" raises the base to base * factor^(c / (c - 1)),
+    which interpolates the slowest pair by factor and leaves the fastest; "parts"
+    interpolates a pair by how often it turns over the ``trained`` positions: whole
+    below ``slow`` turns, not at all above ``fast``, in between in proportion, and
+    gives the magnitude 0.1 ln(factor) + 1 (Peng et al., YaRN, 2023)."""
+    pairs = (pairs,) if type(pairs) is int else tuple(pairs)
+    if not 1 <= len(pairs) <= 3 or any(type(c) is not int or c < 0 for c in pairs) or sum(pairs) < 1:
+        raise ValueError("pairs must be one to three counts of rotary pairs")
+    if scaling not in SCALINGS:
+        raise ValueError("scaling must be none, linear, ntk or parts")
+    if not (math.isfinite(base) and base > 1 and math.isfinite(factor) and factor >= 1):
+        raise ValueError("base must be above 1 and factor at least 1")
+    if scaling == "parts" and not (trained is not None and trained > 0 and fast > slow > 0):
+        raise ValueError("scaling by parts needs the trained length, and fast > slow > 0")
+    made, magnitude = [], 1.0
+    for count in pairs:
+        j = torch.arange(count, dtype=torch.float64)
+        b = base * factor ** (count / max(1, count - 1)) if scaling == "ntk" else base
+        freq = b ** (-j / max(1, count))
+        if scaling == "linear":
+            freq = freq / factor
+        elif scaling == "parts":
+            kept = ((trained * freq / (2 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+            freq = freq * kept + freq / factor * (1.0 - kept)
+            magnitude = 0.1 * math.log(factor) + 1.0
+        made.append(freq)
+    return torch.cat(made), magnitude
+
+
+def _plan(tensors, positions, freqs, pairs, layout, magnitude):
+    """Checks of apply_rotary's arguments; the argument block without the tensors."""
+    first = tensors[0]
+    if not 1 <= len(tensors) <= MAX_TENSORS:
+        raise ValueError("apply_rotary takes one to four tensors")
+    if any(t.ndim != 4 or t.dtype != first.dtype or t.device != first.device or t.shape[0] != first.shape[0]
+           or t.shape[2:] != first.shape[2:] for t in tensors):
+        raise ValueError("tensors must be [batch, heads, tokens, head_dim] of one type, alike but for the heads")
+    _lib.require_device(first, "q and k")
+    if first.dtype not in _lib.DTYPES:
+        raise ValueError("apply_rotary takes fp32, fp16 or bf16")
+    b, _, n, d = first.shape
+    if freqs.dtype != torch.float64 or freqs.ndim != 1 or freqs.device != first.device:
+        raise ValueError("freqs must be float64 [pairs] on the tensors' device (rotary_frequencies)")
+    count = freqs.shape[0]
+    if not 1 <= count <= d // 2:
+        raise ValueError("freqs must have 1 to head_dim / 2 pairs")
+    pairs = (count,) if pairs is None else tuple(pairs)
+    if not 1 <= len(pairs) <= 3 or any(type(c) is not int or c < 0 for c in pairs) or sum(pairs) != count:
+        raise ValueError("pairs must give each of one to three axes its count of freqs")
+    if layout not in LAYOUTS:
+        raise ValueError("layout must be interleaved or half")
+    if not math.isfinite(magnitude):
+        raise ValueError("magnitude must be finite")
+    if d > 1024 or any(t.shape[1] * (d // 8 + 2) > 8192 for t in tensors):
+        raise ValueError("head_dim at most 1024, heads * (head_dim / 8 + 2) at most 8192")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.device != first.device:
+        raise ValueError("positions must be int32 or int64 on the tensors' device")
+    axes = len(pairs)
+    p = positions.unsqueeze(-1) if axes == 1 else positions
+    p = p.unsqueeze(0) if p.ndim == 2 else p
+    if p.ndim != 3 or p.shape[0] not in (1, b) or p.shape[1:] != (n, axes):
+        raise ValueError("positions must be [tokens] or [batch, tokens], with an axis dimension last for several axes")
+    a = _lib.RotaryArgs()
+    a.tokens, a.count, a.batch, a.head_dim, a.pairs, a.axes = n, len(tensors), b, d, count, axes
+    for i, c in enumerate(pairs):
+        a.axis_pairs[i] = c
+    a.positions = p.data_ptr()
+    a.pos_sb, a.pos_sn, a.pos_sa = (0 if p.shape[0] == 1 else p.stride(0)), p.stride(1), p.stride(2)
+    freqs = freqs.contiguous()
+    a.freqs = freqs.data_ptr()
+    a.pos_is64, a.half, a.dtype = int(p.dtype == torch.int64), int(layout == "half"), _lib.DTYPES[first.dtype]
+    a.magnitude = magnitude
+    return a, freqs
+
+
+def _turn(plan, tensors, inverse):
+    """The tensors turned, each as a [B, H, N, d] view of a [B, N, H, d] buffer."""
+    outs = []
+    plan.inverse = inverse
+    for i, t in enumerate(tensors):
+        if t.stride(-1) != 1:
+            t = t.contiguous()
+        b, h, n, d = t.shape
+        out = torch.empty(b, n, h, d, dtype=t.dtype, device=t.device).transpose(1, 2)
+        plan.x[i], plan.y[i], plan.heads[i] = _lib.view(t), _lib.view(out), h
+        outs.append((out, t))
+    if tensors[0].numel():
+        _lib.launch("p3d_rotary", tensors[0].device, plan)
+    return tuple(out for out, _ in outs)
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, plan, positions, freqs, *tensors):
+        ctx.plan = plan
+        ctx.save_for_backward(positions, freqs)
+        return _turn(plan, tensors, 0)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        ctx.saved_tensors  # raises where positions or freqs were changed since the forward
+        need = [i for i in range(len(grads)) if ctx.needs_input_grad[3 + i]]
+        plan = _lib.RotaryArgs.from_buffer_copy(ctx.plan)
+        plan.count = len(need)
+        back = dict(zip(need, _turn(plan, [grads[i] for i in need], 1)))
+        return (None, None, None, *(back.get(i) for i in range(len(grads))))
+
+
+def apply_rotary(tensors, positions, freqs, *, pairs=None, layout="interleaved", magnitude=1.0):
+    """Queries and keys turned to their positions: one tensor [batch, heads, tokens,
+    head_dim] or a sequence of up to four alike but for their heads (any strides with
+    contiguous channels, such as views of the projections); a tensor or a tuple comes
+    back, as transposed views of [batch, tokens, heads, head_dim] buffers.
+
+    positions: int32 or int64 [tokens] or [batch, tokens]; for several axes of
+    coordinates [..., tokens, axes] with ``pairs`` giving each axis its share of the
+    pairs.  freqs: float64 [P], radians a position, on the device; 2P channels of a
+    head turn, channels 2j and 2j + 1 (interleaved) or j and P + j (half), and are
+    multiplied by magnitude; the rest are copied.  Angles are formed in 64 bits.
+    Differentiable in the tensors (first order)."""
+    one = isinstance(tensors, torch.Tensor)
+    tensors = (tensors,) if one else tuple(tensors)
+    plan, freqs = _plan(tensors, positions, freqs, pairs, layout, float(magnitude))
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        outs = _Rotary.apply(plan, positions, freqs, *tensors)
+    else:
+        outs = _turn(plan, tensors, 0)
+    return outs[0] if one else outs
+
+
+@dataclass(frozen=True)
+class RotaryEncoding:
+    """How ``PACK3DAttention(rotary=...)`` turns q, kl and kg: the coordinates (or, with
+    position_encoding="packed", the packed rows) as positions, ``fraction`` of each
+    head's pairs turned, layout and scaling as in apply_rotary and
+    rotary_frequencies (trained: positions an axis had in training)."""
+
+    layout: str = "interleaved"
+    fraction: float = 1.0
+    base: float = 10000.0
+    scaling: str = "none"
+    factor: float = 1.0
+    trained: float | None = None
+
+    def __post_init__(self):
+        if self.layout not in LAYOUTS:
+            raise ValueError("layout must be interleaved or half")
+        if not 0.0 < self.fraction <= 1.0:
+            raise ValueError("fraction must be in (0, 1]")
+        rotary_frequencies(1, base=self.base, scaling=self.scaling, factor=self.factor, trained=self.trained)
+
+    def pairs(self, head_dim, axes):
+        total = max(axes, int(head_dim // 2 * self.fraction))
+        return tuple(total // axes + (a < total % axes) for a in range(axes))
+
+    def frequencies(self, head_dim, axes, device):
+        """(pairs, frequencies on the device, magnitude)."""
+        pairs = self.pairs(head_dim, axes)
+
+        def make():
+            freqs, magnitude = rotary_frequencies(pairs, base=self.base, scaling=self.scaling, factor=self.factor,
+                                                  trained=self.trained)
+            return freqs.to(device), magnitude
+        return (pairs, *_cached(("rotary", self, pairs, str(device)), make))

@@ -1,0 +1,327 @@
+"""block_norm and block_residual against their definition in 64 bits: outputs, every
+gradient, the kinds of gates, widths from 1 to 8192, strides, empty inputs, values that
+are not finite, a captured graph, another stream."""
+import pytest
+import torch
+
+import pack3d_amd as p3d
+from tests._block_reference import (assert_within, block_reference, half_step, keep_mask, smallest, sum_bound)
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _rand(gen, *shape, dtype=F32, std=1.0, mean=0.0):
+    return (torch.randn(*shape, generator=gen) * std + mean).to(dtype)
+
+
+def _case(gpu, batch, tokens, dim, outer, inner, post, after, gate, scale, alpha, p, param=None, seed=0, grads=True):
+    """Inputs of one call on the device, and what the definition gives for them."""
+    gen = torch.Generator().manual_seed(seed + dim * 31 + tokens)
+    param = param or (inner if outer == inner else F32)
+    rows = batch * tokens
+    t = {"x": _rand(gen, batch, tokens, dim, dtype=outer, std=1.5, mean=0.2), "y": _rand(gen, batch, tokens, dim, dtype=inner)}
+    for name, kind in (("", post), ("next_", after)):
+        if kind:
+            t[name + "weight"] = _rand(gen, dim, dtype=param, std=0.1, mean=1.0)
+            if kind == "layer":
+                t[name + "bias"] = _rand(gen, dim, dtype=param, std=0.1)
+    shape = {"sample": (batch, 1, dim), "shared": (1, 1, dim), "token": (batch, tokens, 1), "full": (batch, tokens, dim)}
+    if gate:
+        t["gate"] = _rand(gen, *shape[gate], dtype=inner, std=0.4, mean=0.5)
+    if scale:
+        t["scale"] = _rand(gen, dim, dtype=param, std=0.2, mean=0.5)
+    up = {"out": _rand(gen, batch, tokens, dim, dtype=outer)}
+    if after:
+        up["n"] = _rand(gen, batch, tokens, dim, dtype=inner)
+    seeds = (0x1234567890ABCDEF + seed, 5 + seed)
+    threshold = int(p * 65536 + 0.5)
+
+    def wide(name):
+        return None if name not in t else t[name].double()
+
+    def norm(kind, pre):
+        return (kind, wide(pre + "weight"), wide(pre + "bias"), 1e-5) if kind else None
+    g = None if not gate else t["gate"].double().expand(batch, tokens, dim).reshape(rows, dim)
+    keep = keep_mask(rows * dim, threshold, *seeds).view(rows, dim) if p else None
+    ref = block_reference(wide("x").view(rows, dim), wide("y").view(rows, dim), norm(post, ""), g, wide("scale"), alpha,
+                          keep, threshold / 65536, norm(after, "next_"),
+                          up["out"].double().view(rows, dim) if grads else None,
+                          up["n"].double().view(rows, dim) if grads and after else None)
+    if grads and gate:
+        terms, dterms = (v.view(batch, tokens, dim) for v in ref.pop("d_gate_terms"))
+        axes = [i for i, (a, b) in enumerate(zip(shape[gate], (batch, tokens, dim))) if a != b]
+        if axes:
+            bound = sum_bound(terms, dterms, rows * (1 if axes[0] < 2 else 0) + dim * (axes[-1] == 2), axes).reshape(shape[gate])
+            ref["d_gate"] = (terms.sum(axes, keepdim=True), bound)
+        else:
+            ref["d_gate"] = (terms, dterms)
+    dev = {k: v.to(gpu) for k, v in t.items()}
+    upd = {k: v.to(gpu) for k, v in up.items()}
+    return dev, upd, ref, seeds
+
+
+def _call(dev, post, after, alpha, p, seeds):
+    def norm(kind, pre):
+        return p3d.Norm(kind, dev[pre + "weight"], dev.get(pre + "bias"), 1e-5) if kind else None
+    got = p3d.block_residual(dev["x"], dev["y"], post_norm=norm(post, ""), gate=dev.get("gate"), scale=dev.get("scale"),
+                             alpha=alpha, p=p, seed=seeds, next_norm=norm(after, "next_"))
+    return {"out": got[0], "n": got[1]} if after else {"out": got}
+
+
+def _check(name, got, ref):
+    value, bound = ref
+    assert_within(got.reshape(value.shape), value,
+                  bound + (half_step(got.dtype) * (value.abs() + bound) + smallest(got.dtype)), name)
+
+
+def _run_case(gpu, post, after, alpha, p, *args, **kw):
+    batch, tokens, dim, outer, inner, gate, scale = args
+    dev, up, ref, seeds = _case(gpu, batch, tokens, dim, outer, inner, post, after, gate, scale, alpha, p, **kw)
+    with torch.no_grad():
+        plain = _call(dev, post, after, alpha, p, seeds)
+    for t in dev.values():
+        t.requires_grad_()
+    outs = _call(dev, post, after, alpha, p, seeds)
+    for k in outs:
+        assert torch.equal(outs[k], plain[k]), k  # with and without a graph
+        _check(k, outs[k], ref[k])
+    grads = torch.autograd.grad(list(outs.values()), list(dev.values()), [up[k] for k in outs])
+    for name, g in zip(dev, grads):
+        assert g.dtype == dev[name].dtype and g.shape == dev[name].shape
+        _check("d_" + name, g, ref["d_" + name])
+
+
+TYPES = [(F32, F32), (F16, F16), (BF16, BF16), (F32, F16), (F32, BF16)]
+
+
+@pytest.mark.parametrize("outer,inner", TYPES)
+@pytest.mark.parametrize("post,after,gate,scale,alpha,p", [
+    (None, None, None, False, 1.0, 0.0),
+    ("layer", "layer", "sample", True, 1.0, 0.1),
+    ("rms", "rms", "token", True, 1.5, 0.0),
+    ("rms", None, "full", False, 1.0, 0.3),
+    (None, "layer", "full", True, 0.5, 0.1),
+    ("layer", None, "token", False, 1.0, 0.25),
+    (None, "rms", "sample", False, 1.0, 0.0),
+    ("layer", "rms", "shared", True, 2.0, 0.5),
+    (None, None, "sample", True, 1.0, 0.1),
+])
+def test_residual_kinds(gpu, outer, inner, post, after, gate, scale, alpha, p):
+    _run_case(gpu, post, after, alpha, p, 3, 37, 72, outer, inner, gate, scale)
+
+
+@pytest.mark.parametrize("dim", [1, 2, 7, 8, 9, 63, 64, 65, 128, 131, 192, 256, 327, 512, 513, 1000, 1024, 1500, 2048, 2049,
+                                 4096, 5001, 8191, 8192])
+def test_residual_widths(gpu, dim):
+    print(f"block_residual dim {dim}", flush=True)
+    _run_case(gpu, "layer", "rms", 1.25, 0.1, 2, 5, dim, F32, BF16, "sample", True)
+    _run_case(gpu, "rms", "layer", 1.0, 0.2, 1, 3, dim, F16, F16, "token", True)
+
+
+@pytest.mark.parametrize("batch,tokens", [(1, 1), (1, 2), (7, 1), (1, 999), (600, 3), (5000, 1), (2, 4099), (1, 40000)])
+def test_residual_rows(gpu, batch, tokens):
+    _run_case(gpu, "rms", "layer", 1.0, 0.1, batch, tokens, 40, F32, BF16, "sample", True)
+    _run_case(gpu, None, None, 1.0, 0.0, batch, tokens, 40, BF16, BF16, "sample", False)
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("outer,inner", TYPES)
+@pytest.mark.parametrize("rows,dim", [(1, 4096), (3, 1), (300, 192), (77, 515), (4000, 64), (9, 8192)])
+def test_block_norm(gpu, kind, outer, inner, rows, dim):
+    gen = torch.Generator().manual_seed(rows + dim)
+    x = _rand(gen, rows, dim, dtype=outer, std=2.0, mean=1.0)
+    w, b = _rand(gen, dim, std=0.1, mean=1.0), _rand(gen, dim, std=0.1)
+    dn = _rand(gen, rows, dim, dtype=inner)
+    ref = block_reference(x.double(), None, None, None, None, 1.0, None, 0.0, (kind, w.double(), b.double(), 1e-6), None,
+                          dn.double())
+    x, w, b = (t.to(gpu).requires_grad_() for t in (x, w, b))
+    n = p3d.block_norm(x, p3d.Norm(kind, w, b, 1e-6), dtype=inner)
+    assert n.dtype == inner
+    _check("n", n, ref["n"])
+    for name, g in zip(("d_x", "d_next_weight", "d_next_bias"), torch.autograd.grad(n, (x, w, b), dn.to(gpu))):
+        _check(name, g, ref[name])
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+def test_block_norm_without_affine_and_from_modules(gpu, kind):
+    gen = torch.Generator().manual_seed(3)
+    x = _rand(gen, 2, 50, 96, dtype=BF16).to(gpu).requires_grad_()
+    dn = _rand(gen, 2, 50, 96, dtype=BF16).to(gpu)
+    ref = block_reference(x.detach().double().cpu().view(100, 96), None, None, None, None, 1.0, None, 0.0,
+                          (kind, None, None, 1e-5), None, dn.double().cpu().view(100, 96))
+    n = p3d.block_norm(x, p3d.Norm(kind))
+    _check("n", n, ref["n"])
+    _check("d_x", torch.autograd.grad(n, x, dn)[0], ref["d_x"])
+    module = (torch.nn.LayerNorm(96) if kind == "layer" else torch.nn.RMSNorm(96, eps=1e-5)).to(gpu)
+    assert torch.equal(p3d.block_norm(x, p3d.Norm.of(module)), n)
+
+
+def test_a_full_step_agrees_with_differences(gpu):
+    """The gradients of fp32 inputs against central differences of the definition in 64 bits along
+    random directions: a difference of step 1e-5 is off by its third derivative times 1e-10, far
+    below the 1e-4 of the sum that the gradients' fp32 rounding is allowed."""
+    dev, up, ref, seeds = _case(gpu, 2, 9, 24, F32, F32, "layer", "rms", "sample", True, 1.5, 0.2, grads=True)
+    for t in dev.values():
+        t.requires_grad_()
+    outs = _call(dev, "layer", "rms", 1.5, 0.2, seeds)
+    grads = dict(zip(dev, torch.autograd.grad(list(outs.values()), list(dev.values()), [up[k] for k in outs])))
+    base = {k: v.detach().double().cpu() for k, v in dev.items()}
+    keep = keep_mask(18 * 24, int(0.2 * 65536 + 0.5), *seeds).view(18, 24)
+
+    def loss(t):
+        made = block_reference(t["x"].view(18, 24), t["y"].view(18, 24), ("layer", t["weight"], t["bias"], 1e-5),
+                               t["gate"].expand(2, 9, 24).reshape(18, 24), t["scale"], 1.5, keep,
+                               int(0.2 * 65536 + 0.5) / 65536, ("rms", t["next_weight"], None, 1e-5), None, None)
+        return sum((made[k][0] * up[k].double().cpu().view(18, 24)).sum() for k in ("out", "n"))
+    gen = torch.Generator().manual_seed(8)
+    for name in base:
+        step = torch.randn(base[name].shape, generator=gen, dtype=torch.float64)
+        plus, minus = ({**base, name: base[name] + s * 1e-5 * step} for s in (1, -1))
+        difference = (loss(plus) - loss(minus)) / 2e-5
+        terms = grads[name].double().cpu() * step
+        assert abs(terms.sum() - difference) <= 1e-4 * terms.abs().sum(), name
+
+
+def test_strided_inputs_and_upstream(gpu):
+    """Rows of a wider buffer, channels at odd offsets, expanded rows and expanded gradients: the same bits as
+    contiguous copies."""
+    gen = torch.Generator().manual_seed(4)
+    wide = _rand(gen, 2, 33, 3 * 50 + 1, dtype=BF16).to(gpu)
+    x, y, gate = wide[..., 1:51], wide[..., 51:101], wide[..., 101:]
+    w = _rand(gen, 50, dtype=BF16, mean=1.0).to(gpu)
+
+    def run(x, y, gate, transposed=False):
+        x, y, gate = (t.detach().requires_grad_() for t in (x, y, gate))
+        out, n = p3d.block_residual(x, y, post_norm=p3d.Norm("rms", w), gate=gate, p=0.1, seed=3,
+                                    next_norm=p3d.Norm("layer"))
+        return (out, n, *torch.autograd.grad((out, n), (x, y, gate), (torch.ones_like(out) if not transposed else
+                                                                     torch.ones((), dtype=BF16, device=gpu).expand_as(out),
+                                                                     wide[..., 7:57])))
+    for a, b in zip(run(x, y, gate, True), run(*(t.contiguous() for t in (x, y, gate)))):
+        assert torch.equal(a, b)
+    # channels not contiguous, rows expanded
+    xt = _rand(gen, 50, 33, dtype=BF16).to(gpu).t().expand(2, 33, 50)
+    row = y[:, :1].expand(2, 33, 50)
+    for a, b in zip(run(xt, row, gate), run(xt.contiguous(), row.contiguous(), gate)):
+        assert torch.equal(a, b)
+
+
+def test_rows_that_are_not_finite_stay_by_themselves(gpu):
+    """An infinity or NaN shows in its own row of out and n and in no other row, and one that the mask drops
+    does not show at all."""
+    gen = torch.Generator().manual_seed(5)
+    x, y = (_rand(gen, 1, 40, 72).to(gpu) for _ in range(2))
+    clean = p3d.block_residual(x, y, post_norm=p3d.Norm("rms"), next_norm=p3d.Norm("layer"))
+    for value in (float("inf"), float("nan")):
+        bad = y.clone()
+        bad[0, 13, 70] = value
+        got = p3d.block_residual(x, bad, post_norm=p3d.Norm("rms"), next_norm=p3d.Norm("layer"))
+        others = [i for i in range(40) if i != 13]
+        for a, b in zip(got, clean):
+            assert torch.equal(a[0, others], b[0, others])
+            assert not torch.isfinite(a[0, 13]).all()
+    keep = keep_mask(40 * 72, 32768, 9, 0).view(40, 72)
+    bad = torch.where(keep.to(gpu), y[0], float("nan"))[None].requires_grad_()
+    out = p3d.block_residual(x, bad, p=0.5, seed=9)
+    assert torch.isfinite(out).all()
+    (dy,) = torch.autograd.grad(out, bad, torch.ones_like(out))
+    assert torch.equal(dy[0] != 0, keep.to(gpu))
+
+
+def test_empty_inputs(gpu):
+    for shape in ((0, 5, 24), (2, 0, 24), (0, 24)):
+        x, y = (torch.zeros(shape, device=gpu, requires_grad=True) for _ in range(2))
+        w = torch.ones(24, device=gpu, requires_grad=True)
+        out, n = p3d.block_residual(x, y, post_norm=p3d.Norm("rms", w), next_norm=p3d.Norm("layer", w))
+        grads = torch.autograd.grad((out, n), (x, y, w), (out, n))
+        assert out.shape == n.shape == shape and grads[0].shape == shape and not grads[2].any()
+
+
+def test_only_what_is_needed(gpu):
+    """Gradients that nothing asks for are None, and an output that nothing uses counts as zero."""
+    gen = torch.Generator().manual_seed(6)
+    x, y = (_rand(gen, 2, 20, 48).to(gpu).requires_grad_() for _ in range(2))
+    w = (_rand(gen, 48).to(gpu) + 1).requires_grad_()
+    gate = _rand(gen, 2, 1, 48).to(gpu)
+    up = _rand(gen, 2, 20, 48).to(gpu)
+
+    def run():
+        return p3d.block_residual(x, y, post_norm=p3d.Norm("rms", w), gate=gate, next_norm=p3d.Norm("layer", w))
+    out, n = run()
+    only_n = torch.autograd.grad(n, (x, y, w), up)
+    out, n = run()
+    both = torch.autograd.grad((out, n), (x, y, w), (torch.zeros_like(out), up))
+    for a, b in zip(only_n, both):
+        assert torch.equal(a, b)
+    out, n = run()
+    dx, dw = torch.autograd.grad(out, (x, w), up)
+    assert torch.equal(dx, up)
+    plain = p3d.block_residual(x, y, post_norm=p3d.Norm("rms", w), gate=gate)
+    assert torch.equal(torch.autograd.grad(plain, w, up)[0], dw)
+    frozen = p3d.block_residual(x.detach(), y.detach(), post_norm=p3d.Norm("rms", w), gate=gate)
+    assert torch.equal(torch.autograd.grad(frozen, w, up)[0], dw)
+
+
+def test_repeats_bit_for_bit_and_on_another_stream(gpu):
+    def run():
+        dev, up, _, seeds = _case(gpu, 3, 700, 192, F32, BF16, "rms", "layer", "sample", True, 1.0, 0.1, grads=False)
+        for t in dev.values():
+            t.requires_grad_()
+        outs = _call(dev, "rms", "layer", 1.0, 0.1, seeds)
+        return (*outs.values(), *torch.autograd.grad(list(outs.values()), list(dev.values()), [up[k] for k in outs]))
+    first = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = run()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+
+
+def test_training_step_in_a_graph(gpu):
+    """Forward and backward captured once and replayed on new inputs and new seeds, against eager calls."""
+    gen = torch.Generator().manual_seed(7)
+    shape = (2, 65, 80)
+    sets = [[_rand(gen, *shape).to(gpu) for _ in range(3)] for _ in range(3)]
+    seeds = [torch.tensor([11 + i, i], device=gpu) for i in range(3)]
+    w0 = _rand(gen, 80, mean=1.0).to(gpu)
+
+    def step(x, y, up, seed):
+        x, y, w = (t.detach().requires_grad_() for t in (x, y, w0))
+        gate = torch.full((2, 1, 80), 0.5, device=gpu, requires_grad=True)
+        out, n = p3d.block_residual(x, y, post_norm=p3d.Norm("rms", w), gate=gate, p=0.2, seed=seed,
+                                    next_norm=p3d.Norm("layer"))
+        return (out.detach(), n.detach(), *torch.autograd.grad((out, n), (x, y, w, gate), (up, up)))
+    eager = [step(*s, seed) for s, seed in zip(sets, seeds)]
+    held = [t.clone() for t in sets[0]]
+    held_seed = seeds[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*held, held_seed)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*held, held_seed)
+    for i in (0, 1, 2, 0):
+        for h, t in zip(held, sets[i]):
+            h.copy_(t)
+        held_seed.copy_(seeds[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, eager[i]):
+            assert torch.equal(a, b), i
+        step(*sets[1], seeds[1])
+        torch.cuda.synchronize()
+
+
+def test_inputs_changed_before_the_backward_raise(gpu):
+    x, y = (torch.randn(1, 4, 16, device=gpu, requires_grad=True) for _ in range(2))
+    seed = torch.tensor([1, 2], device=gpu)
+    out = p3d.block_residual(x, y, p=0.5, seed=seed)
+    seed.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(out.sum(), x)
