@@ -32,7 +32,8 @@ FLAGS = ["-x", "hip", "-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-fno-honor-nans", "-Wno-nan-infinity-disabled"]
 # Sources whose outputs a loss scaler looks at for what overflowed.
-HONOR_NANS = ("params.hip", "block_fwd.hip", "block_bwd.hip", "dropout.hip", "rotary.hip")
+HONOR_NANS = ("params.hip", "block_f32_f32.hip", "block_f16_f16.hip", "block_bf16_bf16.hip", "block_f32_f16.hip",
+              "block_f32_bf16.hip", "dropout.hip", "rotary.hip")
 
 
 def _hipcc():

@@ -1,19 +1,4 @@
-// What the forward and the backward kernel of a block's end share: the arguments
-// as the device sees them, and how rows are dealt out.
-//
-// Per row of dim channels, all in fp32, each output rounded once:
-//   b = norm1(y) w1 + b1 (or y),  z = keep ? b / (1 - p) : 0,
-//   out = alpha x + scale gate z,  n = norm2(out) w2 + b2,
-// with norm(v) = (v - mean) rstd (LayerNorm, biased variance from the centred
-// values) or v rstd (RMSNorm).  Without y, out is x: the norm before a block.
-//
-// TPR threads share a row and hold eight consecutive channels each; rows of up to
-// 512 channels lie within a wave (several to a wave below), wider ones take a
-// workgroup, so every row is read once into registers whatever its width.
-//
-// Rows are dealt out in units: `tokens` rows that share a gate vector (a sample),
-// cut into `splits` ranges.  A workgroup takes units blockIdx.x, + gridDim.x, ...,
-// so the gate and the parameters stay in registers over a unit's rows.
+// What surrounds a block (block_kernels.hpp) as its kernels see it.
 #pragma once
 
 #include "philox.hpp"
@@ -28,14 +13,13 @@ struct NormDev {
 };
 
 struct BlockDev {
-    int64_t rows, tokens;  // rows = samples * tokens
-    int samples, splits, dim;
+    int64_t tokens;
+    int rows, samples, splits, dim;  // rows = samples * tokens < 2^31
     int param, gate_dtype, gate_kind;
     const void* x;
     const void* y;
-    int64_t x_stride, y_stride;
+    uint32_t x_stride, y_stride, gate_stride;  // bytes between rows (gate: rows or samples)
     const void* gate;
-    int64_t gate_stride;  // elements between rows (full, token) or samples (sample)
     const void* scale;
     float alpha;
     NormDev post, next;
@@ -46,45 +30,16 @@ struct BlockDev {
     // backward
     const void* dout;
     const void* dn;
-    int64_t dout_stride, dn_stride;
+    uint32_t dout_stride, dn_stride;
     void* dx;
     void* dy;
-    void* dgate;       // per token or per element, in gate_dtype
+    void* dgate;        // per token or per element, in gate_dtype
     float* dgate_part;  // [splits][samples][dim], per sample
-    float* part;       // [grid][5][dim]: post weight, post bias, scale, next weight, next bias
+    float* part;        // [grid][5][dim]: post weight, post bias, scale, next weight, next bias
 };
 
-// The rows of unit u: `count` rows from `first` on.
-struct Unit {
-    int sample;
-    int64_t first;
-    int64_t count;
-};
-__device__ __forceinline__ Unit unit_of(const BlockDev& a, int u) {
-    const int split = u / a.samples, sample = u - split * a.samples;
-    const int64_t per = (a.tokens + a.splits - 1) / a.splits;
-    const int64_t at = min(split * per, a.tokens), end = min(at + per, a.tokens);
-    return Unit{sample, sample * a.tokens + at, end - at};
-}
-
-// Threads of a row for a width, and of its workgroup.
-inline int threads_per_row(int dim) {
-    const int pieces = (dim + kPiece - 1) / kPiece;
-    int t = 8;
-    while (t < pieces) t *= 2;
-    return t;
-}
-constexpr int block_threads(int tpr) { return tpr <= 64 ? 256 : tpr; }
-
-// Eight values of a parameter, or `missing` where it has none.
-__device__ __forceinline__ void load_param(const void* p, int dtype, int c, int count, float missing,
-                                           float (&v)[kPiece]) {
-    if (p) load8_any(p, c, dtype, count, v);
-    else
-#pragma unroll
-        for (int e = 0; e < kPiece; ++e) v[e] = missing;
-}
-
-int block_dev(const p3d_block_args* args, BlockDev& a);
+// Launches the kernels of one pair of types (block_<outer>_<inner>.hip).
+template <typename TX, typename TY>
+int launch_block(const BlockDev& a, bool backward, unsigned grid, hipStream_t s);
 
 }  // namespace p3d

@@ -6,8 +6,8 @@
 // (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3, SC
 // 2011) gives for the counter (i / 8, offset) and the key seed.  16 bits an element
 // make the rate a multiple of 2^-16 (what is kept is divided by the rate that the
-// threshold gives, so the mean stays exact) and one block serves the eight
-// elements that a lane holds: 20 products of 32 bits for eight elements.
+// threshold gives, so the mean stays exact) and one block serves eight elements:
+// 20 products of 32 bits for eight elements.
 #pragma once
 
 #include "elements.hpp"
@@ -68,13 +68,41 @@ __device__ __forceinline__ uint32_t keep_group(const MaskDev& m, uint64_t group)
     return bits;
 }
 
-// Bit e set: element first + e stays, e < 8.  Rows of a width that is no multiple
-// of 8 start inside a group and take two of them.
-__device__ __forceinline__ uint32_t keep8(const MaskDev& m, uint64_t first) {
-    const uint32_t shift = (uint32_t)first & 7;
-    uint32_t bits = keep_group(m, first >> 3);
-    if (shift) bits = (bits | keep_group(m, (first >> 3) + 1) << 8) >> shift;
-    return bits & 0xff;
+// Bits of a lane's E elements (at most 8 within a wave, 16 beyond), from channel c of row `row` on, in a tensor of rows
+// of dim.  TPR lanes (every one of them here) hold the row, lane `sub` of them from
+// channel E sub on or less.
+//
+// Where runs of eight and groups coincide each lane computes its own group.  Else the
+// row's groups are dealt out over its lanes and passed between them: a run overlaps two
+// groups, and computing both in each lane took twice the generator's time.  Rows wider
+// than a wave do that all the same.
+template <int TPR, int E>
+__device__ __forceinline__ uint32_t keep_run(const MaskDev& m, uint32_t row, int dim, int c, int sub) {
+    if (E == 8 && dim % 8 == 0) return keep_group(m, (uint64_t)row * (uint32_t)(dim / 8) + (c >> 3));
+    const uint64_t start = (uint64_t)row * (uint32_t)dim;
+    if constexpr (TPR > 64) {
+        const uint64_t first = start + c;
+        const uint32_t shift = (uint32_t)first & 7;
+        uint32_t bits = keep_group(m, first >> 3);
+#pragma unroll
+        for (int k = 1; k < (E + 14) / 8; ++k)
+            if (shift + E > 8 * k) bits |= keep_group(m, (first >> 3) + k) << (8 * k);
+        return bits >> shift;
+    } else {
+        const uint64_t group = start >> 3;
+        const uint32_t at = (uint32_t)(start & 7) + c, g = at >> 3;
+        const uint32_t mine = keep_group(m, group + sub);
+        uint32_t low = __shfl(mine, (int)g, TPR), high = __shfl(mine, (int)g + 1, TPR);
+        // Rows that fill their lanes and start inside a group reach one group past them.
+        if (E * TPR / 8 >= TPR && (at & 7) + E > 8 && g + 1 == TPR) high = keep_group(m, group + TPR);
+        return (low | high << 8) >> (at & 7);
+    }
 }
+
+// Bit e of bits as a word: all ones where it is set.
+__device__ __forceinline__ uint32_t bit_word(uint32_t bits, int e) {
+    return (uint32_t)(((int32_t)(bits << (31 - e))) >> 31);
+}
+__device__ __forceinline__ float and_word(float x, uint32_t w) { return __uint_as_float(__float_as_uint(x) & w); }
 
 }  // namespace p3d

@@ -16,6 +16,7 @@
 namespace p3d {
 namespace {
 
+constexpr int kPiece = 8;
 constexpr int kThreads = 256;
 constexpr int kMaxTensors = 4;
 constexpr int kMaxTable = 4096;  // (cos, sin) of a block: 32 KiB
@@ -36,6 +37,31 @@ struct RotaryDev {
     int half;
     float sign, magnitude;
 };
+
+// v = the first `count` of eight elements at p, zero past them.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int count, float (&v)[kPiece]) {
+    if (count >= kPiece) {
+        Run<T, kPiece> r;
+        r.load(p);
+        r.to(v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) v[e] = e < count ? to_f32(p[e]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int count, const float (&v)[kPiece]) {
+    if (count >= kPiece) {
+        Run<T, kPiece> r;
+        r.from(v);
+        r.store(p);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e)
+            if (e < count) p[e] = from_f32<T>(v[e]);
+    }
+}
 
 // a / d for a < 2^32 / d, with inv = ceil(2^32 / d); d = 1 has inv = 0.
 __device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t inv) { return inv ? __umulhi(a, inv) : a; }

@@ -60,6 +60,7 @@ def _block_args(**kw):
     ({"y": None}, "nothing to compute"), ({"y": None, "scale": 16}, "without y"), ({"y": None, "alpha": 2.0}, "without y"),
     ({"out": None}, "null output"), ({"post": _lib.NormArgs(None, None, 3, 0.0)}, "norm kind"),
     ({"next": _lib.NormArgs(None, None, 1, 0.0)}, "null output"),
+    ({"x_stride": 2 ** 29}, "strides"), ({"y_stride": -1}, "strides"),
     ({"dropout": _lib.Dropout(None, 0, 0, 65536, 0)}, "threshold"), ({"dropout": _lib.Dropout(None, 0, 0, -1, 0)}, "threshold"),
 ])
 def test_block_entry_points_refuse(change, message):
