@@ -596,12 +596,14 @@ typedef struct p3d_norm {
  * statistics that the backward reads: fp32 [4][rows], mean and 1 / sqrt of y (post),
  * then of out (next).
  *
- * Backward (p3d_block_bwd), with the forward's arguments and dout and / or dn: dx,
- * dy and dgate (per token or element, of gate_dtype, contiguous) where they are
- * not NULL; for a gate per sample dgate_part, fp32 [splits][samples][dim], to be
- * summed over the splits; and part, fp32 [grid][5][dim], to be summed over the
- * grid: the gradients of post weight and bias, scale, next weight and bias (rows of
- * parameters that are NULL, and of next without dn, are left as they were).
+ * Backward (p3d_block_bwd), with the forward's arguments, dout (with y) and dn
+ * (or NULL: no gradient through next): dy (with y), dx (with dn; else alpha dout, or
+ * NULL) and dgate (per token or element, contiguous; per sample [samples, dim] or NULL)
+ * of gate_dtype, and the gradients of the parameters d_param[0 .. 4] = post weight and
+ * bias, scale, next weight and bias, [dim] of d_param_dtype[i] each, or NULL (those of
+ * next need dn).  work: fp32 scratch of grid * 5 * dim + splits * samples * dim
+ * elements (the first part where a d_param is asked for, the second for a gate per
+ * sample), in which sums over rows meet before a second launch adds them up.
  *
  * splits: ranges that a sample's rows are cut into, at most `tokens`; grid:
  * workgroups, at most splits * samples. */
@@ -627,8 +629,10 @@ typedef struct p3d_block_args {
     void* dx;
     void* dy;
     void* dgate;
-    float* dgate_part;
-    float* part;
+    void* d_param[5];
+    int32_t d_param_dtype[5];
+    int32_t pad_;
+    float* work;
 } p3d_block_args;
 
 int p3d_block_fwd(const p3d_block_args* args, void* stream);

@@ -103,7 +103,7 @@ class BlockArgs(ctypes.Structure):
                 ("post", NormArgs), ("next", NormArgs), ("dropout", Dropout), ("out", c_void_p), ("n", c_void_p),
                 ("stats", c_void_p), ("dout", c_void_p), ("dn", c_void_p), ("dout_stride", c_int64),
                 ("dn_stride", c_int64), ("dx", c_void_p), ("dy", c_void_p), ("dgate", c_void_p),
-                ("dgate_part", c_void_p), ("part", c_void_p)]
+                ("d_param", c_void_p * 5), ("d_param_dtype", c_int32 * 5), ("pad_", c_int32), ("work", c_void_p)]
 
 
 class RotaryArgs(ctypes.Structure):
@@ -299,11 +299,11 @@ def sum_rows(jobs, device):
 def launch(name, device, *args):
     """``call`` on the device's current stream, with that device current (a
     launch goes to the current device, whatever stream it is given)."""
-    if torch.cuda.current_device() == device.index:
-        call(name, *args, stream_of(device))
-    else:
+    if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
-            call(name, *args, stream_of(device))
+            return call(name, *args, stream_of(device))
+    if getattr(_lib or lib(), name)(*args, stream_of(device)) != 0:
+        raise RuntimeError(f"{name} failed: {lib().p3d_last_error().decode()}")
 
 
 def require_device(t: torch.Tensor, what="tensor"):

@@ -31,6 +31,7 @@ MAX_DIM = 8192
 MAX_STRIDE = 2 ** 29  # elements between rows
 KINDS = {"layer": 1, "rms": 2}  # enum p3d_norm_kind
 SAMPLE, TOKEN, FULL = 1, 2, 3   # enum p3d_gate_kind
+_NO_MASK = _lib.Dropout(None, 0, 0, 0, 0)
 
 
 class Norm(NamedTuple):
@@ -54,6 +55,8 @@ class Norm(NamedTuple):
 
 def _rows(t, dim):
     """t as rows [*, dim] with unit channel stride (a copy where it does not lie so), and the row stride."""
+    if t.is_contiguous():
+        return t, dim
     t = t.reshape(-1, dim)
     if (dim > 1 and t.stride(1) != 1) or t.stride(0) >= MAX_STRIDE:
         t = t.clone(memory_format=torch.contiguous_format)
@@ -62,9 +65,10 @@ def _rows(t, dim):
 
 def _split(samples, tokens, dim, backward):
     """(ranges that a sample's rows are cut into, workgroups)."""
-    threads = next((t for t, most in ((8, 64), (16, 128), (32, 256), (64, 512), (128, 1024), (256, 2048))
-                    if dim <= most), 512)  # of a row
-    rows = max(1, 256 // threads) if threads <= 64 else 1  # that a workgroup holds at a time
+    threads = 8  # of a row
+    while threads < 512 and dim > threads * 8:
+        threads *= 2
+    rows = 256 // threads if threads <= 64 else 1  # that a workgroup holds at a time
     steps = -(-tokens // rows) * samples
     if backward:
         # One round of what the GPU runs at a time (two waves a SIMD): each workgroup
@@ -81,18 +85,18 @@ def _split(samples, tokens, dim, backward):
 
 
 def _check_norm(name, norm, dim, device):
-    if norm is None:
-        return
     if not isinstance(norm, Norm) or norm.kind not in KINDS:
         raise ValueError(f"{name} must be a Norm of kind layer or rms")
-    if not (math.isfinite(norm.eps) and norm.eps >= 0):
+    if not 0 <= norm.eps < math.inf:
         raise ValueError(f"{name}: eps must be finite and not negative")
-    for t in (norm.weight, norm.bias):
-        _check_param(name, t, dim, device)
+    if norm.weight is not None:
+        _check_param(name, norm.weight, dim, device)
+    if norm.bias is not None:
+        _check_param(name, norm.bias, dim, device)
 
 
 def _check_param(name, t, dim, device):
-    if t is not None and (t.shape != (dim,) or t.device != device or not t.is_floating_point()):
+    if t.shape != (dim,) or t.device != device or not t.is_floating_point():
         raise ValueError(f"{name}: parameters must be floating point [dim] on the input's device")
 
 
@@ -112,57 +116,89 @@ def _gate_kind(gate, x):
     raise ValueError("gate must be [batch or 1, 1, dim], [batch, tokens, 1] or [batch, tokens, dim]")
 
 
-class _Call:
-    """One forward: the argument block of both directions and what it points into."""
+class _Spec(NamedTuple):
+    """What a call computes, apart from its tensors."""
 
-    def __init__(self, x, y, gate, scale, params, kinds, eps, alpha, mask, gate_kind, inner):
-        dim = x.shape[-1]
-        a = _lib.BlockArgs()
-        self.shape, self.dim, self.args = x.shape, dim, a
-        rows = x.numel() // dim if dim else 0
-        self.rows = rows
-        # Rows that share a gate vector; a gate of batch 1 is shared by all of them.
-        a.samples = gate.shape[0] if gate_kind == SAMPLE and x.ndim == 3 else 1
-        a.tokens = rows // a.samples if rows else 0
-        a.dim = dim
-        a.outer, a.inner = _lib.DTYPES[x.dtype], _lib.DTYPES[inner]
-        given = [t for t in (*params, scale) if t is not None]
-        dtype = given[0].dtype if given and all(t.dtype == given[0].dtype for t in given) else torch.float32
-        dtype = dtype if dtype in _lib.DTYPES else torch.float32
-        a.param = _lib.DTYPES[dtype]
-        self.keep = [None if t is None else t.to(dtype).contiguous() for t in (*params, scale)]
-        w1, b1, w2, b2, sc = (_lib.ptr(t) for t in self.keep)
-        a.post, a.next = _lib.NormArgs(w1, b1, kinds[0], eps[0]), _lib.NormArgs(w2, b2, kinds[1], eps[1])
-        a.scale, a.alpha, a.dropout = sc, alpha, mask
-        self.bind(x, y, gate)
-        a.gate_kind = gate_kind
-        self.inner = inner
+    kinds: tuple      # of the post and the next norm, 0 where there is none
+    eps: tuple
+    alpha: float
+    mask: object      # ctypes block of the dropout mask
+    gate_kind: int
+    inner: torch.dtype
 
-    def bind(self, x, y, gate):
-        """Points the arguments at x, y and the gate."""
-        a, dim = self.args, self.dim
-        x, a.x_stride = _rows(x, dim)
-        a.x = x.data_ptr()
-        self.tensors = [x]
-        if y is not None:
-            y, a.y_stride = _rows(y, dim)
-            a.y = y.data_ptr()
-            self.tensors.append(y)
-        if gate is not None:
-            gate, a.gate_stride = _rows(gate, gate.shape[-1])
-            a.gate, a.gate_dtype = gate.data_ptr(), _lib.DTYPES[gate.dtype]
-            self.tensors.append(gate)
 
-    def forward(self, x, has_y, save):
-        a, dev = self.args, x.device
-        out = torch.empty(self.shape, dtype=x.dtype, device=dev) if has_y else None
-        n = torch.empty(self.shape, dtype=self.inner, device=dev) if a.next.kind else None
-        stats = torch.empty(4, self.rows, dtype=torch.float32, device=dev) if save else None
-        if self.rows:
-            a.out, a.n, a.stats = _lib.ptr(out), _lib.ptr(n), _lib.ptr(stats)
-            a.splits, a.grid = _split(a.samples, a.tokens, self.dim, False)
-            _lib.launch("p3d_block_fwd", dev, a)
-        return out, n, stats
+def _bind(spec, x, y, gate, scale, params):
+    """The argument block of both directions, without outputs; and what it points into
+    besides the tensors given (copies of those that do not lie as the kernels read them)."""
+    a, keep = _lib.BlockArgs(), []
+    dim = x.shape[-1]
+    rows = x.numel() // dim
+    dtypes = _lib.DTYPES
+    a.dim, a.alpha, a.dropout = dim, spec.alpha, spec.mask
+    a.outer, a.inner = dtypes[x.dtype], dtypes[spec.inner]
+    t, a.x_stride = _rows(x, dim)
+    a.x = t.data_ptr()
+    keep.append(t)
+    if y is not None:
+        t, a.y_stride = _rows(y, dim)
+        a.y = t.data_ptr()
+        keep.append(t)
+    samples = 1  # runs of rows that share a gate vector; a gate of batch 1 is shared by all of them
+    if gate is not None:
+        if spec.gate_kind == SAMPLE and x.ndim == 3:
+            samples = gate.shape[0]
+        t, a.gate_stride = _rows(gate, gate.shape[-1])
+        a.gate, a.gate_dtype, a.gate_kind = t.data_ptr(), dtypes[gate.dtype], spec.gate_kind
+        keep.append(t)
+    a.samples, a.tokens = samples, rows // samples
+    given = [t for t in (*params, scale) if t is not None]
+    if given:
+        # One type for all: their own, or fp32, which holds each of them exactly.
+        dtype = given[0].dtype
+        if dtype not in dtypes or any(t.dtype != dtype for t in given):
+            dtype = torch.float32
+        a.param = dtypes[dtype]
+        at = []
+        for t in (*params, scale):
+            if t is not None and (t.dtype != dtype or not t.is_contiguous()):
+                t = t.to(dtype).contiguous()
+                keep.append(t)
+            at.append(None if t is None else t.data_ptr())
+        w1, b1, w2, b2, a.scale = at
+    else:
+        w1 = b1 = w2 = b2 = None
+    kinds, eps = spec.kinds, spec.eps
+    if kinds[0]:
+        a.post = _lib.NormArgs(w1, b1, kinds[0], eps[0])
+    if kinds[1]:
+        a.next = _lib.NormArgs(w2, b2, kinds[1], eps[1])
+    return a, keep
+
+
+def _empty(like, dtype):
+    """A contiguous tensor of like's shape."""
+    if like.is_contiguous():
+        return torch.empty_like(like, dtype=dtype)
+    return torch.empty(like.shape, dtype=dtype, device=like.device)
+
+
+def _forward(spec, x, y, gate, scale, params, save):
+    """(out or None, n or None, statistics or None)."""
+    a, keep = _bind(spec, x, y, gate, scale, params)
+    rows = a.samples * a.tokens
+    out = None if y is None else _empty(x, x.dtype)
+    n = _empty(x, spec.inner) if spec.kinds[1] else None
+    stats = torch.empty(4, rows, dtype=torch.float32, device=x.device) if save else None
+    if rows:
+        if out is not None:
+            a.out = out.data_ptr()
+        if n is not None:
+            a.n = n.data_ptr()
+        if save:
+            a.stats = stats.data_ptr()
+        a.splits, a.grid = _split(a.samples, a.tokens, a.dim, False)
+        _lib.launch("p3d_block_fwd", x.device, a)
+    return out, n, stats
 
 
 class _Block(torch.autograd.Function):
@@ -170,11 +206,10 @@ class _Block(torch.autograd.Function):
     the rows' statistics; the backward forms out again from x and y."""
 
     @staticmethod
-    def forward(ctx, x, y, gate, scale, w1, b1, w2, b2, state, made):
-        call = _Call(x, y, gate, scale, (w1, b1, w2, b2), *made)
-        out, n, stats = call.forward(x, y is not None, True)
+    def forward(ctx, x, y, gate, scale, w1, b1, w2, b2, state, spec):
+        out, n, stats = _forward(spec, x, y, gate, scale, (w1, b1, w2, b2), True)
         ctx.save_for_backward(x, y, gate, scale, w1, b1, w2, b2, state, stats)
-        ctx.made = made
+        ctx.spec = spec
         ctx.set_materialize_grads(False)
         return (out, n) if out is not None and n is not None else (n if out is None else out)
 
@@ -182,81 +217,70 @@ class _Block(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, *grads):
         x, y, gate, scale, w1, b1, w2, b2, state, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        has_next = bool(ctx.made[0][1])
+        need, spec = ctx.needs_input_grad, ctx.spec
         dout, dn = grads if len(grads) == 2 else ((None, grads[0]) if y is None else (grads[0], None))
-        none = (None,) * 10
         if dout is None and dn is None:
-            return none
-        params = (w1, b1, scale, w2, b2)
-        wanted = [t is not None and need[i] for t, i in zip(params, (4, 5, 3, 6, 7))]
-        alpha, gate_kind = ctx.made[2], ctx.made[4]
-        call = _Call(x, y, gate, scale, (w1, b1, w2, b2), *ctx.made)
-        a, dim, dev, f32 = call.args, call.dim, x.device, torch.float32
+            return (None,) * 10
+        a, keep = _bind(spec, x, y, gate, scale, (w1, b1, w2, b2))
+        dim, dev, rows = a.dim, x.device, a.samples * a.tokens
         # Without a gradient through the next norm dx is alpha dout: dout itself for 1.
-        through = dn is None and alpha == 1.0
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] and not through else None
-        dy = torch.empty(y.shape, dtype=y.dtype, device=dev) if y is not None and need[1] else None
-        dgate = part = dgate_part = None
-        if gate is not None and need[2] and gate_kind != SAMPLE:
-            dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
-        sums = []
-        if call.rows:
+        through = dn is None and spec.alpha == 1.0
+        dx = None if through or not (need[0] or dn is not None) else _empty(x, x.dtype)
+        dy = None if y is None else _empty(y, y.dtype)
+        dgate = None
+        if gate is not None and (need[2] or spec.gate_kind != SAMPLE):
+            dgate = _empty(gate, gate.dtype)
+        dparams = [None] * 5
+        for i, (t, at) in enumerate(((w1, 4), (b1, 5), (scale, 3), (w2, 6), (b2, 7))):
+            if t is not None and need[at]:
+                if not rows or (i >= 3 and dn is None):
+                    dparams[i] = torch.zeros_like(t)
+                    continue
+                g = torch.empty_like(t, dtype=t.dtype if t.dtype in _lib.DTYPES else torch.float32)
+                a.d_param[i], a.d_param_dtype[i] = g.data_ptr(), _lib.DTYPES[g.dtype]
+                dparams[i] = g if g.dtype == t.dtype else (g, t.dtype)
+        if rows:
             a.splits, a.grid = _split(a.samples, a.tokens, dim, True)
-            if gate is not None and need[2] and gate_kind == SAMPLE:
-                dgate_part = torch.empty(a.splits, a.samples * dim, dtype=f32, device=dev)
-                dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
-                sums.append((dgate_part, dgate))
-            if any(wanted):
-                part = torch.empty(a.grid, 5, dim, dtype=f32, device=dev)
-            keep = []
-            for name, t, dtype in (("dout", dout, x.dtype), ("dn", dn, call.inner)):
-                if t is not None:
-                    t, stride = _rows(t.to(dtype), dim)
-                    keep.append(t)
-                    setattr(a, name, t.data_ptr())
-                    setattr(a, name + "_stride", stride)
-            a.stats, a.dx, a.dy, a.part = stats.data_ptr(), _lib.ptr(dx), _lib.ptr(dy), _lib.ptr(part)
-            a.dgate_part = _lib.ptr(dgate_part)
-            a.dgate = _lib.ptr(dgate) if gate_kind in (TOKEN, FULL) else None
-            if dx is not None or dy is not None or dgate is not None or part is not None:
-                _lib.launch("p3d_block_bwd", dev, a)
-        elif gate is not None and need[2]:
-            dgate = torch.zeros_like(gate)
-        out = [None] * 5
-        for i, (t, want) in enumerate(zip(params, wanted)):
-            if not want:
-                continue
-            if not call.rows or (i >= 3 and dn is None):
-                out[i] = torch.zeros_like(t)
-                continue
-            out[i] = torch.empty(dim, dtype=t.dtype if t.dtype in _lib.DTYPES else f32, device=dev)
-            sums.append((part[:, i], out[i]))
-        if sums:
-            with torch.cuda.device(dev):
-                _lib.sum_rows(sums, dev)
-        dw1, db1, dscale, dw2, db2 = (g if g is None else g.to(t.dtype) for g, t in zip(out, params))
-        if through and need[0]:
-            dx = dout
-        return dx, dy, dgate, dscale, dw1, db1, dw2, db2, None, None
+            work = torch.empty((a.grid * 5 + (a.splits * a.samples if spec.gate_kind == SAMPLE else 0)) * dim,
+                               dtype=torch.float32, device=dev)
+            if y is not None:
+                if dout is None:  # only n was used: a row of zeros, for every row
+                    dout = torch.zeros(1, dim, dtype=x.dtype, device=dev).expand(rows, dim)
+                dout, a.dout_stride = _rows(dout if dout.dtype == x.dtype else dout.to(x.dtype), dim)
+                a.dout, a.dy = dout.data_ptr(), dy.data_ptr()
+            if dn is not None:
+                dn, a.dn_stride = _rows(dn if dn.dtype == spec.inner else dn.to(spec.inner), dim)
+                a.dn = dn.data_ptr()
+            if dx is not None:
+                a.dx = dx.data_ptr()
+            if dgate is not None:
+                a.dgate = dgate.data_ptr()
+            a.stats, a.work = stats.data_ptr(), work.data_ptr()
+            _lib.launch("p3d_block_bwd", dev, a)
+        elif dgate is not None:
+            dgate.zero_()
+        dw1, db1, dscale, dw2, db2 = (g[0].to(g[1]) if type(g) is tuple else g for g in dparams)
+        return (None if not need[0] else grads[0] if through else dx, dy if need[1] else None,
+                dgate if need[2] else None, dscale, dw1, db1, dw2, db2, None, None)
 
 
 def _run(x, y, gate, scale, post, after, alpha, p, seed, inner):
-    mask, state = mask_args(p, seed, x.device)
+    mask, state = mask_args(p, seed, x.device) if p != 0.0 else (_NO_MASK, None)
     gate_kind = _gate_kind(gate, x)
-    norms = [n if n is not None else Norm() for n in (post, after)]
-    kinds = [0 if n is None else KINDS[n.kind] for n in (post, after)]
-    params = [t for n in norms for t in (n.weight, n.bias)]
-    made = (kinds, [n.eps for n in norms], alpha, mask, gate_kind, inner)
-    inputs = (x, y, gate, scale, *params)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
-        return _Block.apply(*inputs, state, made)
-    out, n, _ = _Call(x, y, gate, scale, params, *made).forward(x, y is not None, False)
-    return (out, n) if out is not None and n is not None else (n if out is None else out)
+    w1, b1, w2, b2 = params = ((None, None) if post is None else post[1:3]) + ((None, None) if after is None else after[1:3])
+    spec = _Spec((0 if post is None else KINDS[post.kind], 0 if after is None else KINDS[after.kind]),
+                 (0.0 if post is None else post.eps, 0.0 if after is None else after.eps), alpha, mask, gate_kind, inner)
+    if torch.is_grad_enabled():
+        for t in (x, y, gate, scale, *params):
+            if t is not None and t.requires_grad:
+                return _Block.apply(x, y, gate, scale, w1, b1, w2, b2, state, spec)
+    out, n, _ = _forward(spec, x, y, gate, scale, params, False)
+    return n if out is None else out if n is None else (out, n)
 
 
 def _check_x(x):
-    _lib.require_device(x, "x")
+    if not x.is_cuda:
+        _lib.require_device(x, "x")
     if x.dtype not in _lib.DTYPES:
         raise ValueError("x must be fp32, fp16 or bf16")
     if x.ndim not in (2, 3) or not 1 <= x.shape[-1] <= MAX_DIM:
@@ -270,8 +294,6 @@ def block_norm(x, norm: Norm, *, dtype=None):
     fp32 x also fp16 or bf16, as the next products take it): statistics in fp32, one
     rounding, any row stride.  Differentiable in x and the norm's parameters."""
     _check_x(x)
-    if norm is None:
-        raise ValueError("block_norm needs a Norm")
     _check_norm("norm", norm, x.shape[-1], x.device)
     dtype = x.dtype if dtype is None else dtype
     if dtype not in _lib.DTYPES or (x.dtype != torch.float32 and dtype != x.dtype):
@@ -295,9 +317,12 @@ def block_residual(x, y, *, post_norm: Optional[Norm] = None, gate=None, scale=N
     if y.dtype not in _lib.DTYPES or (x.dtype != torch.float32 and y.dtype != x.dtype):
         raise ValueError("y must have x's type, or fp16 or bf16 over an fp32 x")
     dim = x.shape[-1]
-    _check_norm("post_norm", post_norm, dim, x.device)
-    _check_norm("next_norm", next_norm, dim, x.device)
-    _check_param("scale", scale, dim, x.device)
+    if post_norm is not None:
+        _check_norm("post_norm", post_norm, dim, x.device)
+    if next_norm is not None:
+        _check_norm("next_norm", next_norm, dim, x.device)
+    if scale is not None:
+        _check_param("scale", scale, dim, x.device)
     alpha = float(alpha)
     if not math.isfinite(alpha):
         raise ValueError("alpha must be finite")

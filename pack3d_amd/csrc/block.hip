@@ -71,8 +71,6 @@ int block_dev(const p3d_block_args* args, BlockDev& a) {
     a.dx = g.dx;
     a.dy = g.dy;
     a.dgate = g.dgate;
-    a.dgate_part = g.dgate_part;
-    a.part = g.part;
     return P3D_OK;
 }
 
@@ -101,11 +99,33 @@ extern "C" int p3d_block_fwd(const p3d_block_args* args, void* stream) {
 extern "C" int p3d_block_bwd(const p3d_block_args* args, void* stream) {
     BlockDev a;
     if (const int rc = block_dev(args, a)) return rc;
-    P3D_REQUIRE(a.dout || a.dn, "no upstream gradient");
+    P3D_REQUIRE(a.y ? a.dout != nullptr : a.dn != nullptr, "the upstream gradient is missing");
     P3D_REQUIRE(!a.dn || a.next.kind, "a gradient of n needs the next norm");
     P3D_REQUIRE((!a.post.kind && !a.dn) || a.stats, "the norms' statistics are missing");
-    P3D_REQUIRE(!a.dgate || a.gate_kind == P3D_GATE_TOKEN || a.gate_kind == P3D_GATE_FULL, "dgate is per token or element");
-    P3D_REQUIRE(!a.dgate_part || a.gate_kind == P3D_GATE_SAMPLE, "dgate_part is per sample");
-    P3D_REQUIRE(a.y || !a.dy, "dy without y");
-    return launch(*args, a, true, stream);
+    const p3d_block_args& g = *args;
+    const bool gated = a.gate_kind == P3D_GATE_TOKEN || a.gate_kind == P3D_GATE_FULL;
+    P3D_REQUIRE((!a.y || a.dy) && (!a.dn || a.dx) && (!gated || a.dgate), "null output");
+    P3D_REQUIRE(a.gate_kind || !a.dgate, "dgate without a gate");
+    // Where the sums over rows go: a row of the five parameters' a workgroup, a row of
+    // the gate's a unit.
+    p3d_sum_job jobs[6];
+    int count = 0;
+    const void* params[5] = {a.post.weight, a.post.bias, a.scale, a.next.weight, a.next.bias};
+    float* part = g.work;
+    for (int i = 0; i < 5; ++i) {
+        if (!g.d_param[i]) continue;
+        P3D_REQUIRE(params[i] && known(g.d_param_dtype[i]) && (i < 3 || a.dn), "d_param without its parameter or gradient");
+        jobs[count++] = p3d_sum_job{part + (int64_t)i * a.dim, g.d_param[i], g.grid, 5 * (int64_t)a.dim, a.dim,
+                                    g.d_param_dtype[i]};
+    }
+    if (count) a.part = part;
+    if (a.gate_kind == P3D_GATE_SAMPLE && a.dgate) {
+        P3D_REQUIRE((int64_t)a.samples * a.dim < (1LL << 31), "samples * dim out of range");
+        a.dgate_part = part + (count ? (int64_t)g.grid * 5 * a.dim : 0);
+        const int64_t cols = (int64_t)a.samples * a.dim;
+        jobs[count++] = p3d_sum_job{a.dgate_part, a.dgate, a.splits, cols, (int32_t)cols, a.gate_dtype};
+    }
+    P3D_REQUIRE(!count || g.work, "work is missing");
+    if (const int rc = launch(g, a, true, stream)) return rc;
+    return count ? p3d_sum_rows(jobs, count, stream) : P3D_OK;
 }

@@ -142,12 +142,12 @@ template <int E>
 struct GateRun {
     AnyRun<E> r;
     __device__ __forceinline__ void load(const BlockDev& a, uint32_t row, int c) {
-        const uint64_t at = row_address(reinterpret_cast<uint64_t>(a.gate), row, a.gate_stride);
+        const char* at = row_address(reinterpret_cast<const char*>(a.gate), row, a.gate_stride);
         if (a.gate_kind == P3D_GATE_TOKEN) {
             r.raw[0] = a.gate_dtype == P3D_F32 ? *reinterpret_cast<const uint32_t*>(at)
                                                : (uint32_t)*reinterpret_cast<const uint16_t*>(at);
         } else {
-            r.load(reinterpret_cast<const void*>(at), a.gate_dtype, c);
+            r.load(at, a.gate_dtype, c);
         }
     }
     __device__ __forceinline__ void to(const BlockDev& a, float (&g)[E]) const {
@@ -198,8 +198,10 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_fwd(BlockDev a) {
     const float inv_dim = 1.f / (float)a.dim;
     MaskDev mask = a.mask;
     mask_begin(mask);
-    const uint64_t px = reinterpret_cast<uint64_t>(a.x) + c * sizeof(TX), py = reinterpret_cast<uint64_t>(a.y) + c * sizeof(TY);
-    const uint64_t pout = reinterpret_cast<uint64_t>(a.out) + c * sizeof(TX), pn = reinterpret_cast<uint64_t>(a.n) + c * sizeof(TY);
+    const char* px = reinterpret_cast<const char*>(a.x) + c * sizeof(TX);
+    const char* py = reinterpret_cast<const char*>(a.y) + c * sizeof(TY);
+    char* pout = reinterpret_cast<char*>(a.out) + c * sizeof(TX);
+    char* pn = reinterpret_cast<char*>(a.n) + c * sizeof(TY);
     float par[4][E];
     load_params<E, 4>({a.next.weight, a.next.bias, HAS_Y ? a.post.weight : nullptr, HAS_Y ? a.post.bias : nullptr}, a.param,
                       c, {1.f, 0.f, 1.f, 0.f}, par);
@@ -221,8 +223,8 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_fwd(BlockDev a) {
         Run<TY, E> yr;
         GateRun<E> gr;
         auto fetch = [&](uint32_t row) {
-            xr.load(reinterpret_cast<const void*>(row_address(px, row, a.x_stride)));
-            if constexpr (HAS_Y) yr.load(reinterpret_cast<const void*>(row_address(py, row, a.y_stride)));
+            xr.load(row_address(px, row, a.x_stride));
+            if constexpr (HAS_Y) yr.load(row_address(py, row, a.y_stride));
             if constexpr (GATED) gr.load(a, row, c);
         };
         const int last = unit.count - 1;
@@ -259,7 +261,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_fwd(BlockDev a) {
                 if (at.in_row()) {
                     Run<TX, E> o;
                     o.from(v);
-                    o.store(reinterpret_cast<void*>(row_address(pout, row, a.dim * (uint32_t)sizeof(TX))));
+                    o.store(row_address(pout, row, a.dim * (uint32_t)sizeof(TX)));
                 }
             }
             if (a.next.kind) {
@@ -269,7 +271,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_fwd(BlockDev a) {
                 if (at.in_row()) {
                     Run<TY, E> o;
                     o.from(v);
-                    o.store(reinterpret_cast<void*>(row_address(pn, row, a.dim * (uint32_t)sizeof(TY))));
+                    o.store(row_address(pn, row, a.dim * (uint32_t)sizeof(TY)));
                 }
                 if (a.stats && at.sub == 0) {
                     a.stats[2 * (int64_t)a.rows + row] = mean;
@@ -280,7 +282,11 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_fwd(BlockDev a) {
     }
 }
 
-template <typename TX, typename TY, int TPR, int E, int FORM>
+// NEXT: with a gradient of n.  Every load and store of a row but the gate's is made on
+// every path, by every lane (those past the row store their neighbour's bits): the wait
+// for the next row's loads then knows how many stores came after them, and does not wait
+// for the stores.
+template <typename TX, typename TY, int TPR, int E, int FORM, bool NEXT>
 __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
     constexpr int GROUPS = TPR > 64 ? 1 : 256 / TPR;
     constexpr bool HAS_Y = FORM != kNorm, GATED = FORM == kEndGated;
@@ -290,13 +296,16 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
     const int c = at.c;
     const float inv_dim = 1.f / (float)a.dim;
     const bool layer1 = a.post.kind == P3D_NORM_LAYER, layer2 = a.next.kind == P3D_NORM_LAYER;
-    const bool has_dout = a.dout != nullptr, has_dn = a.dn != nullptr, has_post = HAS_Y && a.post.kind;
+    const bool has_post = HAS_Y && a.post.kind;
     const bool per_sample = a.gate_kind == P3D_GATE_SAMPLE;
     MaskDev mask = a.mask;
     mask_begin(mask);
-    const uint64_t px = reinterpret_cast<uint64_t>(a.x) + c * sizeof(TX), py = reinterpret_cast<uint64_t>(a.y) + c * sizeof(TY);
-    const uint64_t pdout = reinterpret_cast<uint64_t>(a.dout) + c * sizeof(TX), pdn = reinterpret_cast<uint64_t>(a.dn) + c * sizeof(TY);
-    const uint64_t pdx = reinterpret_cast<uint64_t>(a.dx) + c * sizeof(TX), pdy = reinterpret_cast<uint64_t>(a.dy) + c * sizeof(TY);
+    const char* px = reinterpret_cast<const char*>(a.x) + c * sizeof(TX);
+    const char* py = reinterpret_cast<const char*>(a.y) + c * sizeof(TY);
+    const char* pdout = reinterpret_cast<const char*>(a.dout) + c * sizeof(TX);
+    const char* pdn = reinterpret_cast<const char*>(a.dn) + c * sizeof(TY);
+    char* pdx = reinterpret_cast<char*>(a.dx) + c * sizeof(TX);
+    char* pdy = reinterpret_cast<char*>(a.dy) + c * sizeof(TY);
     float par[3][E];
     load_params<E, 3>({a.next.weight, HAS_Y ? a.post.weight : nullptr, HAS_Y ? a.post.bias : nullptr}, a.param, c,
                       {1.f, 1.f, 0.f}, par);
@@ -347,20 +356,22 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
             GateRun<E> gr;
             float st[4];  // the row's statistics
             auto fetch = [&](uint32_t row) {
-                if (has_dout) dor.load(reinterpret_cast<const void*>(row_address(pdout, row, a.dout_stride)));
-                if (has_dn) {
-                    xr.load(reinterpret_cast<const void*>(row_address(px, row, a.x_stride)));
-                    dnr.load(reinterpret_cast<const void*>(row_address(pdn, row, a.dn_stride)));
+                if (has_post) {
+                    st[0] = a.stats[row];
+                    st[1] = a.stats[a.rows + row];
+                }
+                if constexpr (NEXT) {
                     st[2] = a.stats[2 * (int64_t)a.rows + row];
                     st[3] = a.stats[3 * (int64_t)a.rows + row];
                 }
+                if constexpr (GATED) gr.load(a, row, c);
                 if constexpr (HAS_Y) {
-                    yr.load(reinterpret_cast<const void*>(row_address(py, row, a.y_stride)));
-                    if constexpr (GATED) gr.load(a, row, c);
-                    if (has_post) {
-                        st[0] = a.stats[row];
-                        st[1] = a.stats[a.rows + row];
-                    }
+                    yr.load(row_address(py, row, a.y_stride));
+                    dor.load(row_address(pdout, row, a.dout_stride));
+                }
+                if constexpr (NEXT) {
+                    xr.load(row_address(px, row, a.x_stride));
+                    dnr.load(row_address(pdn, row, a.dn_stride));
                 }
             };
             const int last = unit.count - 1;
@@ -368,17 +379,17 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
             for (int i = at.grp; i <= last; i += GROUPS) {
                 const uint32_t row = unit.first + i;
                 float go[E], xh2[E], g2[E], xh1[E], g[E];
-                if (has_dout) {
+                if constexpr (HAS_Y) {
+                    yr.to(xh1);
                     dor.to(go);
                 } else {
 #pragma unroll
                     for (int e = 0; e < E; ++e) go[e] = 0.f;
                 }
-                if (has_dn) {
+                if constexpr (NEXT) {
                     xr.to(xh2);
                     dnr.to(g2);
                 }
-                if constexpr (HAS_Y) yr.to(xh1);
                 if constexpr (GATED) gr.to(a, g);
                 const float mean1 = st[0], rstd1 = st[1], mean2 = st[2], rstd2 = st[3];
                 fetch(unit.first + min(i + GROUPS, last));
@@ -401,7 +412,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
                         for (int e = 0; e < E; ++e) b[e] = and_word(b[e], bit_word(bits, e));
                     }
                 }
-                if (has_dn) {
+                if constexpr (NEXT) {
                     float p[E], s[2];
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
@@ -420,13 +431,13 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) go[e] += rstd2 * (g2[e] - m0 - xh2[e] * m1);
                 }
-                if (a.dx && at.in_row()) {
+                if (NEXT || a.dx) {
                     float v[E];
                     Run<TX, E> o;
 #pragma unroll
                     for (int e = 0; e < E; ++e) v[e] = a.alpha * go[e];
                     o.from(v);
-                    o.store(reinterpret_cast<void*>(row_address(pdx, row, a.dim * (uint32_t)sizeof(TX))));
+                    o.store(row_address(pdx, row, a.dim * (uint32_t)sizeof(TX)));
                 }
                 if constexpr (HAS_Y) {
                     float db[E], dg[E], s[GATED ? 3 : 2];
@@ -447,7 +458,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
 #pragma unroll
                         for (int e = 0; e < E; ++e) db[e] = and_word(db[e], bit_word(bits, e));
                     }
-                    const bool token_sum = GATED && a.gate_kind == P3D_GATE_TOKEN && a.dgate;
+                    const bool token_sum = GATED && a.gate_kind == P3D_GATE_TOKEN;
                     if constexpr (GATED) s[2] = token_sum ? at.own(dg) : 0.f;
                     if (has_post) {
                         float p[E];
@@ -467,14 +478,13 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
 #pragma unroll
                         for (int e = 0; e < E; ++e) db[e] = rstd1 * (db[e] - m0 - xh1[e] * m1);
                     }
-                    if (a.dy && at.in_row()) {
-                        Run<TY, E> o;
-                        o.from(db);
-                        o.store(reinterpret_cast<void*>(row_address(pdy, row, a.dim * (uint32_t)sizeof(TY))));
-                    }
+                    Run<TY, E> o;
+                    o.from(db);
+                    o.store(row_address(pdy, row, a.dim * (uint32_t)sizeof(TY)));
                     if constexpr (GATED) {
-                        if (token_sum && at.sub == 0) store_any(a.dgate, row, a.gate_dtype, s[2]);
-                        if (a.dgate && a.gate_kind == P3D_GATE_FULL && at.in_row()) {
+                        if (token_sum) {
+                            store_any(a.dgate, row, a.gate_dtype, s[2]);
+                        } else {
                             const int64_t to = (int64_t)row * a.dim + c;
                             if (a.gate_dtype == P3D_F32) {
                                 Run<float, E> o;
@@ -520,15 +530,20 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
             gather(dsc, part + 2 * a.dim);
         }
     }
-    if (a.next.weight && has_dn) gather(dw2, part + 3 * (int64_t)a.dim);
-    if (a.next.bias && has_dn) gather(db2, part + 4 * (int64_t)a.dim);
+    if (NEXT && a.next.weight) gather(dw2, part + 3 * (int64_t)a.dim);
+    if (NEXT && a.next.bias) gather(db2, part + 4 * (int64_t)a.dim);
 }
 
 template <typename TX, typename TY, int TPR, int E, int FORM>
 int launch_form(const BlockDev& a, bool backward, unsigned grid, hipStream_t s) {
-    if (backward) k_block_bwd<TX, TY, TPR, E, FORM><<<grid, block_threads(TPR), 0, s>>>(a);
-    else k_block_fwd<TX, TY, TPR, E, FORM><<<grid, block_threads(TPR), 0, s>>>(a);
-    return check_launch(backward ? "p3d_block_bwd" : "p3d_block_fwd");
+    constexpr int threads = block_threads(TPR);
+    if (backward) {
+        if (FORM == kNorm || a.dn) k_block_bwd<TX, TY, TPR, E, FORM, true><<<grid, threads, 0, s>>>(a);
+        else k_block_bwd<TX, TY, TPR, E, FORM, FORM == kNorm><<<grid, threads, 0, s>>>(a);
+        return check_launch("p3d_block_bwd");
+    }
+    k_block_fwd<TX, TY, TPR, E, FORM><<<grid, threads, 0, s>>>(a);
+    return check_launch("p3d_block_fwd");
 }
 
 template <typename TX, typename TY, int TPR, int E>

@@ -30,8 +30,13 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, int dtype, float x
     else reinterpret_cast<__bf16*>(p)[i] = (__bf16)x;
 }
 
-// base + row * stride, with both below 2^32: one multiply-add.
-__device__ __forceinline__ uint64_t row_address(uint64_t base, uint32_t row, uint32_t stride) {
+// base + row * stride bytes, with both below 2^32: one multiply-add.  Addresses stay
+// pointers of the kernel's arguments: ones made from integers compile to flat accesses,
+// whose waits are the LDS's too, and no load is then ahead of a reduction.
+__device__ __forceinline__ const char* row_address(const char* base, uint32_t row, uint32_t stride) {
+    return base + (uint64_t)row * stride;
+}
+__device__ __forceinline__ char* row_address(char* base, uint32_t row, uint32_t stride) {
     return base + (uint64_t)row * stride;
 }
 
@@ -43,8 +48,15 @@ __device__ __forceinline__ float group_sum(float x) {
     if constexpr (LANES >= 4) x += dpp_move<0x4E>(x);
     if constexpr (LANES >= 8) x += dpp_move<0x141>(x);
     if constexpr (LANES >= 16) x += dpp_move<0x140>(x);
-    if constexpr (LANES >= 32) x += lane_xor16(x);
-    if constexpr (LANES >= 64) x += lane_xor32(x);
+    // The row swaps give x of the even and of the odd rows (halves), in every lane.
+    if constexpr (LANES >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (LANES >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
     return x;
 }
 

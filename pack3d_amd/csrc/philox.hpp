@@ -35,6 +35,11 @@ __device__ __forceinline__ void mask_begin(MaskDev& m) {
     }
 }
 
+// a ^ b ^ c in one instruction (0x96 is its truth table).
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+    return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+}
+
 // Philox4x32-10 of the counter (group, offset).
 __device__ __forceinline__ void philox(uint64_t group, uint64_t offset, uint64_t seed, uint32_t (&c)[4]) {
     c[0] = (uint32_t)group;
@@ -46,9 +51,9 @@ __device__ __forceinline__ void philox(uint64_t group, uint64_t offset, uint64_t
     for (int r = 0; r < 10; ++r) {
         const uint64_t a = (uint64_t)c[0] * 0xD2511F53u, b = (uint64_t)c[2] * 0xCD9E8D57u;
         const uint32_t c1 = c[1], c3 = c[3];
-        c[0] = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c[0] = xor3((uint32_t)(b >> 32), c1, k0);
         c[1] = (uint32_t)b;
-        c[2] = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c[2] = xor3((uint32_t)(a >> 32), c3, k1);
         c[3] = (uint32_t)a;
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
@@ -99,9 +104,12 @@ __device__ __forceinline__ uint32_t keep_run(const MaskDev& m, uint32_t row, int
     }
 }
 
-// Bit e of bits as a word: all ones where it is set.
+// Bit e of bits as a word: all ones where it is set.  (The instruction by name: the
+// compiler makes a comparison and a select, with a wait between them, of the builtin.)
 __device__ __forceinline__ uint32_t bit_word(uint32_t bits, int e) {
-    return (uint32_t)(((int32_t)(bits << (31 - e))) >> 31);
+    uint32_t w;
+    asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(w) : "v"(bits), "n"(e));
+    return w;
 }
 __device__ __forceinline__ float and_word(float x, uint32_t w) { return __uint_as_float(__float_as_uint(x) & w); }
 

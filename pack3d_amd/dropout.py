@@ -48,9 +48,9 @@ def mask_args(p, seed, device):
 
 
 def _apply(x, mask):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    x = x.contiguous()
+    y = torch.empty_like(x)
     if x.numel():
-        x = x.contiguous()
         _lib.launch("p3d_dropout_apply", x.device, x.data_ptr(), y.data_ptr(), x.numel(), _lib.DTYPES[x.dtype], mask)
     return y
 
@@ -74,7 +74,8 @@ def counter_dropout(x, p, seed):
     others divided by 1 - p.  The same seed gives the same mask, in the backward too;
     another call needs another seed or offset.  fp32, fp16 and bf16, any shape (a
     tensor that is not contiguous is copied first)."""
-    _lib.require_device(x, "x")
+    if not x.is_cuda:
+        _lib.require_device(x, "x")
     if x.dtype not in _lib.DTYPES:
         raise ValueError("counter_dropout takes fp32, fp16 or bf16")
     mask, state = mask_args(p, seed, x.device)

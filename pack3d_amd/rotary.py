@@ -60,65 +60,85 @@ def rotary_frequencies(pairs, *, base=10000.0, scaling="none", factor=1.0, train
 
 
 def _plan(tensors, positions, freqs, pairs, layout, magnitude):
-    """Checks of apply_rotary's arguments; the argument block without the tensors."""
-    first = tensors[0]
+    """Checks of apply_rotary's arguments; the argument block without the tensors, and
+    the frequencies as it points at them."""
     if not 1 <= len(tensors) <= MAX_TENSORS:
         raise ValueError("apply_rotary takes one to four tensors")
-    if any(t.ndim != 4 or t.dtype != first.dtype or t.device != first.device or t.shape[0] != first.shape[0]
-           or t.shape[2:] != first.shape[2:] for t in tensors):
-        raise ValueError("tensors must be [batch, heads, tokens, head_dim] of one type, alike but for the heads")
-    _lib.require_device(first, "q and k")
-    if first.dtype not in _lib.DTYPES:
+    first = tensors[0]
+    shape, dtype, device = first.shape, first.dtype, first.device
+    if len(shape) != 4:
+        raise ValueError("tensors must be [batch, heads, tokens, head_dim]")
+    b, _, n, d = shape
+    for t in tensors:
+        if t.dtype != dtype or t.device != device or t.shape != (b, t.shape[1], n, d):
+            raise ValueError("tensors must be [batch, heads, tokens, head_dim] of one type, alike but for the heads")
+        if not 0 < t.shape[1] * (d // 8 + 2) <= 8192:
+            raise ValueError("heads must be at least 1, heads * (head_dim / 8 + 2) at most 8192")
+    if not first.is_cuda:
+        _lib.require_device(first, "q and k")
+    if dtype not in _lib.DTYPES:
         raise ValueError("apply_rotary takes fp32, fp16 or bf16")
-    b, _, n, d = first.shape
-    if freqs.dtype != torch.float64 or freqs.ndim != 1 or freqs.device != first.device:
+    if freqs.dtype != torch.float64 or freqs.ndim != 1 or freqs.device != device:
         raise ValueError("freqs must be float64 [pairs] on the tensors' device (rotary_frequencies)")
     count = freqs.shape[0]
-    if not 1 <= count <= d // 2:
-        raise ValueError("freqs must have 1 to head_dim / 2 pairs")
-    pairs = (count,) if pairs is None else tuple(pairs)
-    if not 1 <= len(pairs) <= 3 or any(type(c) is not int or c < 0 for c in pairs) or sum(pairs) != count:
-        raise ValueError("pairs must give each of one to three axes its count of freqs")
+    if not 1 <= count <= d // 2 or d > 1024:
+        raise ValueError("freqs must have 1 to head_dim / 2 pairs, head_dim at most 1024")
+    a = _lib.RotaryArgs()
+    axes = 1
+    if pairs is None:
+        a.axis_pairs[0] = count
+    else:
+        axes = len(pairs)
+        if not 1 <= axes <= 3 or sum(pairs) != count:
+            raise ValueError("pairs must give each of one to three axes its count of freqs")
+        for i, c in enumerate(pairs):
+            if type(c) is not int or c < 0:
+                raise ValueError("pairs must be counts")
+            a.axis_pairs[i] = c
     if layout not in LAYOUTS:
         raise ValueError("layout must be interleaved or half")
     if not math.isfinite(magnitude):
         raise ValueError("magnitude must be finite")
-    if d > 1024 or any(t.shape[1] * (d // 8 + 2) > 8192 for t in tensors):
-        raise ValueError("head_dim at most 1024, heads * (head_dim / 8 + 2) at most 8192")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.device != first.device:
+    if positions.dtype not in (torch.int32, torch.int64) or positions.device != device:
         raise ValueError("positions must be int32 or int64 on the tensors' device")
-    axes = len(pairs)
-    p = positions.unsqueeze(-1) if axes == 1 else positions
-    p = p.unsqueeze(0) if p.ndim == 2 else p
-    if p.ndim != 3 or p.shape[0] not in (1, b) or p.shape[1:] != (n, axes):
+    of, strides = positions.shape, positions.stride()
+    if axes == 1:
+        of, strides = (*of, 1), (*strides, 1)
+    if len(of) == 2:
+        of, strides = (1, *of), (0, *strides)
+    if len(of) != 3 or of[0] not in (1, b) or of[1:] != (n, axes):
         raise ValueError("positions must be [tokens] or [batch, tokens], with an axis dimension last for several axes")
-    a = _lib.RotaryArgs()
     a.tokens, a.count, a.batch, a.head_dim, a.pairs, a.axes = n, len(tensors), b, d, count, axes
-    for i, c in enumerate(pairs):
-        a.axis_pairs[i] = c
-    a.positions = p.data_ptr()
-    a.pos_sb, a.pos_sn, a.pos_sa = (0 if p.shape[0] == 1 else p.stride(0)), p.stride(1), p.stride(2)
+    a.positions = positions.data_ptr()
+    a.pos_sb, a.pos_sn, a.pos_sa = 0 if of[0] == 1 else strides[0], strides[1], strides[2]
     freqs = freqs.contiguous()
     a.freqs = freqs.data_ptr()
-    a.pos_is64, a.half, a.dtype = int(p.dtype == torch.int64), int(layout == "half"), _lib.DTYPES[first.dtype]
+    a.pos_is64, a.half, a.dtype = positions.dtype == torch.int64, layout == "half", _lib.DTYPES[dtype]
     a.magnitude = magnitude
     return a, freqs
 
 
 def _turn(plan, tensors, inverse):
     """The tensors turned, each as a [B, H, N, d] view of a [B, N, H, d] buffer."""
-    outs = []
+    first = tensors[0]
+    b, n, d = plan.batch, plan.tokens, plan.head_dim
+    heads = [t.shape[1] for t in tensors]
+    outs, keep = [], []
     plan.inverse = inverse
-    for i, t in enumerate(tensors):
-        if t.stride(-1) != 1:
+    for i, (t, h) in enumerate(zip(tensors, heads)):
+        s = t.stride()
+        if s[3] != 1:
             t = t.contiguous()
-        b, h, n, d = t.shape
-        out = torch.empty(b, n, h, d, dtype=t.dtype, device=t.device).transpose(1, 2)
-        plan.x[i], plan.y[i], plan.heads[i] = _lib.view(t), _lib.view(out), h
-        outs.append((out, t))
-    if tensors[0].numel():
-        _lib.launch("p3d_rotary", tensors[0].device, plan)
-    return tuple(out for out, _ in outs)
+            keep.append(t)
+            s = t.stride()
+        out = torch.empty((b, n, h, d), dtype=first.dtype, device=first.device)
+        plan.x[i] = _lib.View(t.data_ptr(), s[0], s[1], s[2])
+        plan.y[i] = _lib.View(out.data_ptr(), n * h * d, d, h * d)
+        plan.heads[i] = h
+        outs.append(out.transpose(1, 2))
+    if first.numel():
+        _lib.launch("p3d_rotary", first.device, plan)
+    return tuple(outs)
 
 
 class _Rotary(torch.autograd.Function):

@@ -72,9 +72,17 @@ def test_block_entry_points_refuse(change, message):
 
 
 @pytest.mark.parametrize("change,message", [
-    ({}, "upstream"), ({"dn": 16}, "next norm"), ({"dout": 16, "post": _lib.NormArgs(None, None, 1, 0.0)}, "statistics"),
-    ({"dout": 16, "dgate": 16}, "dgate"), ({"dout": 16, "dgate_part": 16}, "dgate_part"),
-    ({"dn": 16, "y": None, "out": None, "dy": 16, "stats": 16, "next": _lib.NormArgs(None, None, 1, 0.0)}, "dy without y"),
+    ({}, "upstream"), ({"dn": 16}, "upstream"), ({"dout": 16, "dn": 16}, "next norm"),
+    ({"dout": 16, "post": _lib.NormArgs(None, None, 1, 0.0)}, "statistics"),
+    ({"dout": 16}, "null output"), ({"dout": 16, "dy": 16, "dgate": 16}, "dgate without"),
+    ({"dout": 16, "dy": 16, "gate": 16, "gate_kind": 2}, "null output"),
+    ({"dout": 16, "dy": 16, "gate": 16, "gate_kind": 1, "dgate": 16}, "work"),
+    ({"dout": 16, "dy": 16, "d_param": (ctypes.c_void_p * 5)(16)}, "d_param without"),
+    ({"dout": 16, "dy": 16, "d_param": (ctypes.c_void_p * 5)(None, None, 16), "scale": 16}, "work"),
+    ({"dout": 16, "dy": 16, "d_param": (ctypes.c_void_p * 5)(None, None, None, 16),
+      "next": _lib.NormArgs(16, None, 1, 0.0)}, "d_param without"),
+    ({"y": None, "out": None, "next": _lib.NormArgs(None, None, 1, 0.0)}, "upstream"),
+    ({"y": None, "out": None, "dn": 16, "stats": 16, "next": _lib.NormArgs(None, None, 1, 0.0)}, "null output"),
 ])
 def test_block_backward_refuses(change, message):
     with pytest.raises(RuntimeError, match=message):
