@@ -20,6 +20,11 @@ rotation, pooling, local and global attention and their fusion run in
 bf16 forward and under autocast over an fp32 input (``p3d_out_residual``;
 otherwise one GEMM with the residual as its C operand).  The projections are
 consumed as strided views, without copies.
+
+Options that the reference's layer does not have: ``rotary`` (a ``RotaryEncoding``: q,
+kl and kg turned by ``apply_rotary`` before the core), and an end of the block with
+``post_norm``, ``layer_scale`` and ``dropout``, a gate per call and the next block's
+norm, all in one pass (``block.block_residual``) in place of ``x + to_out(y)``.
 """
 from __future__ import annotations
 
@@ -29,11 +34,15 @@ import torch
 from torch import nn
 
 from . import _lib
-from .core import SUPPORTED_HEAD_DIMS, ForwardPlan, _projection_views, _validate_inputs, pack3d_hip_projections
+from .block import Norm, block_residual
+from .core import (SUPPORTED_HEAD_DIMS, ForwardPlan, _projection_views, _validate_inputs, pack3d_hip,
+                   pack3d_hip_projections)
+from .dropout import new_seed, threshold_of
 from .linear import (GateProbability, InputProjections, LayerNormTrain, OutputResidual, OutputResidualWide,
                      compute_dtype, fp32_training, layer_norm_train_supported, wide_residual_supported)
 from .geometry import TokenLayout, blocks_consecutive
 from .rope import axial_rope, balanced_pairs, packed_rope
+from .rotary import RotaryEncoding, apply_rotary
 
 
 def layer_norm(norm: nn.LayerNorm, x):
@@ -196,7 +205,12 @@ class PACK3DAttention(nn.Module):
     """Local residual plus gated compressed attention and an outer residual (attention.py:10-21)."""
 
     def __init__(self, dim, *, heads=4, kv_heads=2, head_dim=32, block_volume=8,
-                 backend="hip", position_encoding="axial", temperature=1.0):
+                 backend="hip", position_encoding="axial", temperature=1.0, rotary=None, post_norm=None,
+                 layer_scale=None, dropout=0.0):
+        """rotary: a RotaryEncoding in place of the layer's own rotation; post_norm: "layer" or "rms", the norm
+        of the branch before the residual sum; layer_scale: the initial value of a learned scale per channel
+        on the branch; dropout: its rate on the branch while training.  Without them the layer is the
+        reference's, with its parameters."""
         super().__init__()
         if any(type(v) is not int or v <= 0 for v in (dim, heads, kv_heads, head_dim, block_volume)):
             raise ValueError("dimensions must be positive integers")
@@ -208,7 +222,15 @@ class PACK3DAttention(nn.Module):
             raise ValueError("position_encoding must be axial or packed")
         if not math.isfinite(temperature) or temperature <= 0:
             raise ValueError("temperature must be finite and positive")
+        if rotary is not None and not isinstance(rotary, RotaryEncoding):
+            raise ValueError("rotary must be a RotaryEncoding")
+        if post_norm not in (None, "layer", "rms"):
+            raise ValueError("post_norm must be None, layer or rms")
+        if layer_scale is not None and not math.isfinite(layer_scale):
+            raise ValueError("layer_scale must be finite")
+        threshold_of(dropout)
         self.dim, self.heads, self.kv_heads, self.head_dim = dim, heads, kv_heads, head_dim
+        self.rotary, self.dropout = rotary, float(dropout)
         self.backend, self.position_encoding = backend, position_encoding
         self.temperature = float(temperature)
         # Creation order fixes the RNG stream (attention.py:40-51).
@@ -224,9 +246,16 @@ class PACK3DAttention(nn.Module):
         self.local_scale = nn.Parameter(torch.ones(head_dim))
         self.global_scale = nn.Parameter(torch.full((head_dim,), 0.25))
         self.to_out = nn.Linear(heads * head_dim, dim, bias=False)
+        # After the reference's parameters, so that theirs are drawn alike.
+        self.post_norm = None
+        if post_norm is not None:
+            self.post_norm = nn.LayerNorm(dim) if post_norm == "layer" else nn.RMSNorm(dim, eps=1e-5)
+        self.layer_scale = None if layer_scale is None else nn.Parameter(torch.full((dim,), float(layer_scale)))
 
     def core_inputs(self, x, layout: TokenLayout):
         """Unrotated q, kl, vl, kg, vg (views of the projections), gate, and the rotation."""
+        if self.rotary is not None:
+            raise ValueError("core_inputs gives the layer's own rotation; this layer has a RotaryEncoding")
         b, n = x.shape[0], x.shape[1]
         qp, kvp, gate, _ = self._projections(x)
         q = qp.view(b, n, self.heads, self.head_dim).transpose(1, 2)
@@ -240,11 +269,39 @@ class PACK3DAttention(nn.Module):
             return packed_rope(self.head_dim, n, x.device)
         return axial_rope(self.head_dim, layout.grid_shape, layout.coords, balanced_pairs(self.head_dim))
 
-    def _projections(self, x):
+    def _turned(self, qp, kvp, layout):
+        """q, kl, vl, kg, vg [B, *, N, d] of the projections with q, kl and kg turned by ``self.rotary``."""
+        q, kl, vl, kg, vg = _projection_views(qp, kvp, self.heads, self.kv_heads)
+        axial = self.position_encoding == "axial"
+        positions = layout.coords if axial else torch.arange(qp.shape[1], device=qp.device)
+        pairs, freqs, magnitude = self.rotary.frequencies(self.head_dim, 3 if axial else 1, qp.device)
+        q, kl, kg = apply_rotary((q, kl, kg), positions, freqs, pairs=pairs, layout=self.rotary.layout,
+                                 magnitude=magnitude)
+        return q, kl, vl, kg, vg
+
+    def _normed_projections(self, x, normed):
+        """_projections for tokens that are already normalised."""
+        b, n = x.shape[0], x.shape[1]
+        lin = (self.to_q, self.to_kv, self.gate)
+        dt = compute_dtype(x) if self._hip_linear(x) else None
+        if (dt is None and not torch.is_grad_enabled() and x.is_cuda and x.dtype in (torch.float16, torch.bfloat16)
+                and not torch.is_autocast_enabled("cuda") and all(_plain_linear(m) and m.weight.dtype == x.dtype for m in lin)):
+            dt = x.dtype
+        if dt is not None and self.gate.bias is not None:
+            qp, kvp, gl = InputProjections.apply(normed, self.to_q.weight, self.to_kv.weight, self.gate.weight,
+                                                 self.gate.bias.detach(), dt)
+            gate = GateProbability.apply(gl, self.gate.bias, self.heads,
+                                         torch.float32 if torch.is_autocast_enabled("cuda") else gl.dtype)
+        else:
+            qp, kvp, gl = (m(normed) for m in lin)
+            gate = gl.view(b, n, self.heads, 2).softmax(-1)[..., 1].transpose(1, 2)
+        return qp, kvp, gate
+
+    def _projections(self, x, through=False):
         """qp [B, N, H*d], kvp [B, N, 4*G*d] (kl | vl | kg | vg), the gate
         [B, H, N], and the residual operand of the output product when
         LayerNormTrain wrote it (x rounded to the compute type, [B*N, dim];
-        else None)."""
+        else None); with through, x itself as LayerNormTrain passes it on."""
         b, n = x.shape[0], x.shape[1]
         res = None
         fused = fused_projections(self, x)
@@ -254,7 +311,9 @@ class PACK3DAttention(nn.Module):
         elif self._hip_linear(x):
             dt = compute_dtype(x)
             if layer_norm_train_supported(self.norm, x):
-                if x.dtype == dt:  # the residual copy is the output product's accumulator
+                if through:  # x for block_residual, whose gradient the norm's backward adds
+                    xn, res = LayerNormTrain.apply(x, self.norm.weight, self.norm.bias, self.norm.eps, dt, "pass")
+                elif x.dtype == dt:  # the residual copy is the output product's accumulator
                     xn, res = LayerNormTrain.apply(x, self.norm.weight, self.norm.bias, self.norm.eps, dt, True)
                 elif wide_residual_supported(x, self.heads * self.head_dim, self.dim, dt):
                     # x itself, for the output product's fp32 residual (one consumer of x)
@@ -279,7 +338,27 @@ class PACK3DAttention(nn.Module):
             gate = gl.view(b, n, self.heads, 2).softmax(-1)[..., 1].transpose(1, 2)
         return qp, kvp, gate, res
 
-    def forward(self, x, layout: TokenLayout):
+    def _end(self, x, res, o, gate, next_norm):
+        """The block's end on the core's output o [B*N, H*d]: x or its alias res plus to_out(o) through the
+        post norm, dropout, gate and scale, and the next block's norm."""
+        if self._hip_linear(x) or self._fp32_linear(x):
+            y = OutputResidual.apply(None, o, self.to_out.weight, compute_dtype(x) or torch.float32)
+        else:
+            y = self.to_out(o)
+        if res is not None:
+            x = res.view(x.shape)
+        y = y.view(x.shape)
+        if x.dtype != torch.float32:
+            y = y.to(x.dtype)
+        p = self.dropout if self.training else 0.0
+        return block_residual(x, y, post_norm=None if self.post_norm is None else Norm.of(self.post_norm), gate=gate,
+                              scale=self.layer_scale, p=p, seed=new_seed(x.device) if p else None, next_norm=next_norm)
+
+    def forward(self, x, layout: TokenLayout, *, residual_gate=None, next_norm=None, normed=None):
+        """x plus the block's branch.  residual_gate: a gate on the branch, as block_residual's
+        ([batch, 1, dim] of a conditioned model, or per token or element); next_norm: the next
+        block's norm (a Norm, nn.LayerNorm or nn.RMSNorm), whose result comes back beside the sum;
+        normed: x normalised already, by the block before, with this layer's norm as its next_norm."""
         layout.check_unmodified()
         if x.ndim != 3 or x.shape[0] == 0 or tuple(x.shape[1:]) != (layout.geometry.num_tokens, self.dim):
             raise ValueError("x must be [batch,layout_tokens,dim] with a nonempty batch")
@@ -290,9 +369,23 @@ class PACK3DAttention(nn.Module):
         if self.backend != "hip":
             raise ValueError("unknown backend; implicit fallback is disabled")
         b, n = x.shape[0], x.shape[1]
-        out, res = pooled_core(self, x, layout), None
+        ends = (residual_gate is not None or next_norm is not None or self.post_norm is not None
+                or self.layer_scale is not None or (self.training and self.dropout > 0))
+        if next_norm is not None and not isinstance(next_norm, Norm):
+            next_norm = Norm.of(next_norm)
+        if normed is not None and (normed.shape != x.shape or normed.device != x.device):
+            raise ValueError("normed must have x's shape and device")
+        own = self.rotary is None and normed is None
+        out, res = pooled_core(self, x, layout) if own else None, None
         if out is None:
-            qp, kvp, gate, res = self._projections(x)
+            if normed is not None:
+                qp, kvp, gate = self._normed_projections(x, normed)
+            else:
+                qp, kvp, gate, res = self._projections(x, ends)
+        if out is None and self.rotary is not None:
+            out = pack3d_hip(*self._turned(qp, kvp, layout), self.pool_weight, self.slot_bias, gate, self.local_scale,
+                             self.global_scale, layout.geometry, temperature=self.temperature)
+        elif out is None:
             out = pack3d_hip_projections(qp, kvp, self.heads, self.kv_heads, self.pool_weight, self.slot_bias,
                                          gate, self.local_scale, self.global_scale, layout.geometry,
                                          self._rope(x, layout), temperature=self.temperature)
@@ -300,6 +393,8 @@ class PACK3DAttention(nn.Module):
         # residual as its C operand (to_out has no bias), with a HIP weight gradient
         # in 16-bit training.
         o = out.transpose(1, 2).reshape(b * n, -1)
+        if ends:
+            return self._end(x, res, o, residual_gate, next_norm)
         fused = fused_out_residual(self, x, o)
         if fused is not None:
             return fused.view(b, n, self.dim)

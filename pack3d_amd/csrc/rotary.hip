@@ -8,9 +8,15 @@
 // distance from the nearest whole turn is rounded to 32 bits, an error of at most
 // 2^-26 turns.
 //
-// A block takes a run of tokens: first (cos, sin) of each of their pairs into LDS,
-// once for all heads of all tensors, then the heads, 8 pairs (32 bytes of a 16-bit
-// type) a thread and step.  Bound by memory: 4 bytes an element in 16 bits.
+// A block takes a run of tokens: (cos, sin) of each of their pairs into LDS, once for
+// all heads of all tensors, then the heads, eight pairs (32 bytes of a 16-bit type) or
+// eight copied channels a thread and step, the first step's loads issued before the
+// angles are worked out.  A block takes the tokens of one step a thread: more blocks with
+// smaller tables measured faster than steps ahead within one (three bf16 tensors of
+// 262,144 x 4 x 48: 124 us; with two steps a thread 126, four 136, their loads together
+// 140), and the angles cost nothing next to the memory (138 and 139 us without and with
+// them).  Where eight does not divide the pairs, the last two steps of a head overlap and
+// store the same bits twice.  Bound by memory: 4 bytes an element in 16 bits, 4.9 TB/s.
 #include "elements.hpp"
 
 namespace p3d {
@@ -23,54 +29,129 @@ constexpr int kMaxTable = 4096;  // (cos, sin) of a block: 32 KiB
 
 struct RotaryDev {
     p3d_view x[kMaxTensors], y[kMaxTensors];
-    uint32_t items[kMaxTensors];        // heads * chunks of a token
-    uint32_t items_inv[kMaxTensors];    // ceil(2^32 / items)
+    uint32_t steps[kMaxTensors];        // of a token
+    uint32_t steps_inv[kMaxTensors];    // ceil(2^32 / steps)
     int count;
-    int64_t tokens, tiles;              // tiles of a batch entry
+    int64_t tokens;
+    uint32_t tiles;                     // of a batch entry
     int run;                            // tokens of a tile
-    int head_dim, pairs, chunks, turned;  // chunks of a head, of which `turned` hold pairs
-    uint32_t chunks_inv;
+    int head_dim, pairs;
+    uint32_t chunks, turned, chunks_inv;  // steps of a head, of which `turned` hold pairs
     const void* positions;
     int64_t pb, pn, pa;                 // strides of the positions
-    int pos64, axes, end0, end1;        // pairs below end0 are on axis 0, below end1 on axis 1
+    int pos64, end0, end1;              // pairs below end0 are on axis 0, below end1 on axis 1
     const double* freqs;
-    int half;
     float sign, magnitude;
 };
-
-// v = the first `count` of eight elements at p, zero past them.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int count, float (&v)[kPiece]) {
-    if (count >= kPiece) {
-        Run<T, kPiece> r;
-        r.load(p);
-        r.to(v);
-    } else {
-#pragma unroll
-        for (int e = 0; e < kPiece; ++e) v[e] = e < count ? to_f32(p[e]) : 0.f;
-    }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int count, const float (&v)[kPiece]) {
-    if (count >= kPiece) {
-        Run<T, kPiece> r;
-        r.from(v);
-        r.store(p);
-    } else {
-#pragma unroll
-        for (int e = 0; e < kPiece; ++e)
-            if (e < count) p[e] = from_f32<T>(v[e]);
-    }
-}
 
 // a / d for a < 2^32 / d, with inv = ceil(2^32 / d); d = 1 has inv = 0.
 __device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t inv) { return inv ? __umulhi(a, inv) : a; }
 
-template <typename T>
+// One step: sixteen channels that turn (two runs of eight, apart or adjacent), or eight
+// that are copied.  SMALL: heads with fewer than eight pairs, or with one to seven
+// channels to copy, whose runs are shorter than eight.
+template <typename T, bool HALF, bool SMALL>
+struct Step {
+    const char* src;
+    char* dst;
+    uint32_t at;  // of the (cos, sin) of its first pair
+    int count;    // pairs, or minus the channels to copy
+    Run<T, kPiece> u, v;
+
+    // k: the tensor, the same for the whole launch's step.
+    __device__ __forceinline__ void place(const RotaryDev& a, int k, int64_t b, int64_t first, uint32_t i) {
+        const uint32_t t = quotient(i, a.steps_inv[k]), r = i - t * a.steps[k];
+        const uint32_t h = quotient(r, a.chunks_inv), c = r - h * a.chunks;
+        const p3d_view &x = a.x[k], &y = a.y[k];
+        const int P = a.pairs, left = a.head_dim - 2 * P;
+        int64_t channel;
+        if (c < a.turned) {
+            const int j = SMALL ? (int)c * kPiece : min((int)c * kPiece, P - kPiece);
+            at = t * P + j;
+            count = SMALL ? min(kPiece, P - j) : kPiece;
+            channel = HALF ? j : 2 * j;
+        } else {
+            const int j = (int)(c - a.turned) * kPiece;
+            at = 0;
+            count = -min(kPiece, left - j);
+            channel = SMALL ? 2 * P + j : min(2 * P + j, a.head_dim - kPiece);
+        }
+        src = reinterpret_cast<const char*>(reinterpret_cast<const T*>(x.data) + b * x.sb + (int64_t)h * x.sh +
+                                            (first + t) * x.sn + channel);
+        dst = reinterpret_cast<char*>(reinterpret_cast<T*>(y.data) + b * y.sb + (int64_t)h * y.sh +
+                                      (first + t) * y.sn + channel);
+    }
+    // Bytes from the first run of eight channels to the second.
+    __device__ __forceinline__ int64_t apart(const RotaryDev& a) const {
+        return (HALF ? a.pairs : kPiece) * (int64_t)sizeof(T);
+    }
+    __device__ __forceinline__ static void load_some(Run<T, kPiece>& r, const char* p, int n) {
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) r.v[e] = e < n ? reinterpret_cast<const T*>(p)[e] : from_f32<T>(0.f);
+    }
+    __device__ __forceinline__ static void store_some(const Run<T, kPiece>& r, char* p, int n) {
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e)
+            if (e < n) reinterpret_cast<T*>(p)[e] = r.v[e];
+    }
+    // Channels of the two runs, in the small form.
+    __device__ __forceinline__ int first_run() const { return count < 0 ? -count : (HALF ? count : min(2 * count, kPiece)); }
+    __device__ __forceinline__ int second_run() const { return count < 0 ? 0 : (HALF ? count : 2 * count - kPiece); }
+    __device__ __forceinline__ void load(const RotaryDev& a) {
+        if constexpr (SMALL) {
+            load_some(u, src, first_run());
+            load_some(v, src + apart(a), second_run());
+        } else {
+            u.load(src);
+            // A step that copies reads its own run twice rather than none: no branch.
+            v.load(src + (count < 0 ? 0 : apart(a)));
+        }
+    }
+    __device__ __forceinline__ void turn(const RotaryDev& a, const float2* table) {
+        if (count > 0) {
+            float f[kPiece], g[kPiece];
+            u.to(f);
+            v.to(g);
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) {
+                const float2 w = table[at + (SMALL && e >= count ? 0 : e)];
+                float& p = HALF ? f[e] : (e < kPiece / 2 ? f[(2 * e) % kPiece] : g[(2 * e) % kPiece]);
+                float& q = HALF ? g[e] : (e < kPiece / 2 ? f[(2 * e + 1) % kPiece] : g[(2 * e + 1) % kPiece]);
+                const float s = p * w.x - q * w.y, t = p * w.y + q * w.x;
+                p = s;
+                q = t;
+            }
+            u.from(f);
+            v.from(g);
+        }
+        if constexpr (SMALL) {
+            store_some(u, dst, first_run());
+            store_some(v, dst + apart(a), second_run());
+        } else {
+            if (count == -kPiece || count > 0) {
+                u.store(dst);
+                if (count > 0) v.store(dst + apart(a));
+            } else {
+#pragma unroll
+                for (int e = 0; e < kPiece; ++e)
+                    if (e >= kPiece + count) reinterpret_cast<T*>(dst)[e] = u.v[e];
+            }
+        }
+    }
+};
+
+template <typename T, bool HALF, bool SMALL>
 __global__ __launch_bounds__(kThreads) void k_rotary(RotaryDev a) {
-    __shared__ float2 table[kMaxTable];
-    const int64_t b = blockIdx.x / a.tiles, first = (blockIdx.x - b * a.tiles) * a.run;
+    extern __shared__ float2 table[];  // [run][pairs]
+    const uint32_t entry = blockIdx.x / a.tiles;
+    const int64_t b = entry, first = (int64_t)(blockIdx.x - entry * a.tiles) * a.run;
     const int live = (int)min((int64_t)a.run, a.tokens - first);
+    Step<T, HALF, SMALL> s;
+    auto fetch = [&](int k, uint32_t i, uint32_t all) {
+        s.place(a, k, b, first, min(i, all - 1));  // past the end: the last step once more
+        s.load(a);
+    };
+    fetch(0, threadIdx.x, (uint32_t)live * a.steps[0]);
     for (int i = threadIdx.x; i < live * a.pairs; i += kThreads) {
         const int t = i / a.pairs, j = i - t * a.pairs;
         const int axis = j < a.end0 ? 0 : (j < a.end1 ? 1 : 2);
@@ -79,63 +160,33 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryDev a) {
                                     : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[at];
         const double turns = (double)pos * (a.freqs[j] * 0.15915494309189533577);  // 1 / (2 pi)
         const float r = (float)(turns - rint(turns));
-        float s, c;
-        sincospif(2.f * r, &s, &c);
-        table[i] = float2{c * a.magnitude, s * a.magnitude * a.sign};
+        float sn, cs;
+        sincospif(2.f * r, &sn, &cs);
+        table[i] = float2{cs * a.magnitude, sn * a.magnitude * a.sign};
     }
     __syncthreads();
     for (int k = 0; k < a.count; ++k) {
-        const uint32_t items = a.items[k], all = (uint32_t)live * items;
-        const T* xb = reinterpret_cast<const T*>(a.x[k].data) + b * a.x[k].sb;
-        T* yb = reinterpret_cast<T*>(a.y[k].data) + b * a.y[k].sb;
-        for (uint32_t i = threadIdx.x; i < all; i += kThreads) {
-            const uint32_t t = quotient(i, a.items_inv[k]), r = i - t * items;
-            const uint32_t h = quotient(r, a.chunks_inv), c = r - h * a.chunks;
-            const T* xr = xb + (int64_t)h * a.x[k].sh + (first + t) * a.x[k].sn;
-            T* yr = yb + (int64_t)h * a.y[k].sh + (first + t) * a.y[k].sn;
-            if ((int)c >= a.turned) {
-                const int at = 2 * a.pairs + ((int)c - a.turned) * kPiece, n = min(kPiece, a.head_dim - at);
-                float v[kPiece];
-                load8(xr + at, n, v);
-                store8(yr + at, n, v);
-                continue;
-            }
-            const int j = (int)c * kPiece, n = min(kPiece, a.pairs - j);
-            const float2* cs = table + t * a.pairs + j;
-            float u[kPiece], v[kPiece];
-            if (a.half) {
-                load8(xr + j, n, u);
-                load8(xr + a.pairs + j, n, v);
-#pragma unroll
-                for (int e = 0; e < kPiece; ++e) {
-                    const float2 w = cs[e < n ? e : 0];
-                    const float p = u[e] * w.x - v[e] * w.y, q = u[e] * w.y + v[e] * w.x;
-                    u[e] = p;
-                    v[e] = q;
-                }
-                store8(yr + j, n, u);
-                store8(yr + a.pairs + j, n, v);
-            } else {
-                load8(xr + 2 * j, min(2 * n, kPiece), u);
-                load8(xr + 2 * j + kPiece, 2 * n - kPiece, v);
-#pragma unroll
-                for (int e = 0; e < kPiece / 2; ++e) {
-                    const float2 w = cs[e < n ? e : 0], z = cs[e + kPiece / 2 < n ? e + kPiece / 2 : 0];
-                    const float p = u[2 * e] * w.x - u[2 * e + 1] * w.y, q = u[2 * e] * w.y + u[2 * e + 1] * w.x;
-                    const float f = v[2 * e] * z.x - v[2 * e + 1] * z.y, g = v[2 * e] * z.y + v[2 * e + 1] * z.x;
-                    u[2 * e] = p;
-                    u[2 * e + 1] = q;
-                    v[2 * e] = f;
-                    v[2 * e + 1] = g;
-                }
-                store8(yr + 2 * j, min(2 * n, kPiece), u);
-                store8(yr + 2 * j + kPiece, 2 * n - kPiece, v);
-            }
+        const uint32_t all = (uint32_t)live * a.steps[k];
+        if (k) fetch(k, threadIdx.x, all);
+        for (uint32_t i = threadIdx.x;;) {
+            if (i < all) s.turn(a, table);
+            i += kThreads;
+            if (i >= all) break;
+            fetch(k, i, all);
         }
     }
 }
 
 inline uint32_t inverse_of(uint32_t d) { return d == 1 ? 0 : (uint32_t)(((1ULL << 32) + d - 1) / d); }
+
+template <typename T>
+void launch(const RotaryDev& a, bool half, bool small, unsigned blocks, hipStream_t s) {
+    const size_t lds = (size_t)a.run * a.pairs * sizeof(float2);
+    if (half && small) k_rotary<T, true, true><<<blocks, kThreads, lds, s>>>(a);
+    else if (half) k_rotary<T, true, false><<<blocks, kThreads, lds, s>>>(a);
+    else if (small) k_rotary<T, false, true><<<blocks, kThreads, lds, s>>>(a);
+    else k_rotary<T, false, false><<<blocks, kThreads, lds, s>>>(a);
+}
 
 }  // namespace
 }  // namespace p3d
@@ -154,54 +205,55 @@ extern "C" int p3d_rotary(const p3d_rotary_args* args, void* stream) {
     const int axes = g.axes;
     int sum = 0;
     for (int i = 0; i < axes; ++i) {
-        P3D_REQUIRE(g.axis_pairs[i] >= 0, "axis pairs must not be negative");
+        P3D_REQUIRE(g.axis_pairs[i] >= 0 && g.axis_pairs[i] <= g.pairs, "axis pairs must add up to pairs");
         sum += g.axis_pairs[i];
     }
     P3D_REQUIRE(sum == g.pairs, "axis pairs must add up to pairs");
     RotaryDev a{};
-    a.count = g.count;
     a.tokens = g.tokens;
     a.head_dim = g.head_dim;
     a.pairs = g.pairs;
-    a.turned = (int)cdiv(g.pairs, kPiece);
-    a.chunks = a.turned + (int)cdiv(g.head_dim - 2 * g.pairs, kPiece);
+    const int left = g.head_dim - 2 * g.pairs;
+    a.turned = (uint32_t)cdiv(g.pairs, kPiece);
+    a.chunks = a.turned + (uint32_t)cdiv(left, kPiece);
     a.chunks_inv = inverse_of(a.chunks);
-    uint32_t per_token = 0;
+    a.count = g.count;
+    uint32_t most = 0;
     for (int k = 0; k < g.count; ++k) {
         P3D_REQUIRE(g.x[k].data && g.y[k].data && g.heads[k] >= 1, "null tensor or no heads");
         P3D_REQUIRE((int64_t)g.heads[k] * a.chunks <= 8192, "heads * head_dim too large");
         a.x[k] = g.x[k];
         a.y[k] = g.y[k];
-        a.items[k] = (uint32_t)(g.heads[k] * a.chunks);
-        a.items_inv[k] = inverse_of(a.items[k]);
-        per_token += a.items[k];
+        a.steps[k] = (uint32_t)g.heads[k] * a.chunks;
+        a.steps_inv[k] = inverse_of(a.steps[k]);
+        most = most > a.steps[k] ? most : a.steps[k];
     }
     a.positions = g.positions;
     a.pb = g.pos_sb;
     a.pn = g.pos_sn;
     a.pa = g.pos_sa;
     a.pos64 = g.pos_is64;
-    a.axes = axes;
     a.end0 = axes > 1 ? g.axis_pairs[0] : g.pairs;
     a.end1 = axes > 2 ? g.axis_pairs[0] + g.axis_pairs[1] : g.pairs;
     a.freqs = g.freqs;
-    a.half = g.half;
     a.sign = g.inverse ? -1.f : 1.f;
     a.magnitude = g.magnitude;
-    // Tokens of a block: about four steps of its threads, within the table, and
-    // fewer where that leaves CUs without a block.
-    int64_t run = cdiv(4 * kThreads, per_token);
+    // Tokens of a block: a step a thread of the tensor with most heads, within the table,
+    // and fewer where that leaves CUs without a block.
+    int64_t run = kThreads / most;
+    run = run < 1 ? 1 : run;
     run = run < kMaxTable / g.pairs ? run : kMaxTable / g.pairs;
     while (run > 1 && g.batch * cdiv(g.tokens, run) < 512) run = (run + 1) / 2;
     a.run = (int)run;
-    a.tiles = cdiv(g.tokens, run);
-    P3D_REQUIRE(g.batch * a.tiles < (1LL << 31), "launch grid too large");
-    const unsigned blocks = (unsigned)(g.batch * a.tiles);
+    P3D_REQUIRE(g.batch * cdiv(g.tokens, run) < (1LL << 31), "launch grid too large");
+    a.tiles = (uint32_t)cdiv(g.tokens, run);
+    const unsigned blocks = (unsigned)g.batch * a.tiles;
+    const bool small = g.pairs < kPiece;
     hipStream_t s = as_stream(stream);
     switch (g.dtype) {
-        case P3D_F32: k_rotary<float><<<blocks, kThreads, 0, s>>>(a); break;
-        case P3D_F16: k_rotary<_Float16><<<blocks, kThreads, 0, s>>>(a); break;
-        default: k_rotary<__bf16><<<blocks, kThreads, 0, s>>>(a); break;
+        case P3D_F32: launch<float>(a, g.half, small, blocks, s); break;
+        case P3D_F16: launch<_Float16>(a, g.half, small, blocks, s); break;
+        default: launch<__bf16>(a, g.half, small, blocks, s); break;
     }
     return check_launch("p3d_rotary");
 }
