@@ -183,7 +183,7 @@ def _empty(like, dtype):
 
 
 def _forward(spec, x, y, gate, scale, params, save):
-    """(out or None, n or None, statistics or None)."""
+    """(out or None, n or None, the argument block with what it points into, statistics or None)."""
     a, keep = _bind(spec, x, y, gate, scale, params)
     rows = a.samples * a.tokens
     out = None if y is None else _empty(x, x.dtype)
@@ -198,7 +198,38 @@ def _forward(spec, x, y, gate, scale, params, save):
             a.stats = stats.data_ptr()
         a.splits, a.grid = _split(a.samples, a.tokens, a.dim, False)
         _lib.launch("p3d_block_fwd", x.device, a)
-    return out, n, stats
+    return out, n, (a, keep), stats
+
+
+def _still(a, x, y, gate, scale, params):
+    """Whether an argument block points at these very tensors (saved tensors may come back as others)."""
+    if a.x != x.data_ptr() or a.y != (None if y is None else y.data_ptr()):
+        return False
+    post, after = a.post, a.next
+    for at, t in ((a.gate, gate), (a.scale, scale), (post.weight, params[0]), (post.bias, params[1]),
+                  (after.weight, params[2]), (after.bias, params[3])):
+        if at != (None if t is None else t.data_ptr()):
+            return False
+    return True
+
+
+def _param_grads(a, params, wanted, dim):
+    """Gradients of the parameters that are wanted, in the order of the argument block, and
+    their addresses entered there: one allocation where they have one type."""
+    which = [i for i in range(5) if wanted[i]]
+    grads = [None] * 5
+    if not which:
+        return grads
+    dtype = params[which[0]].dtype
+    if dtype in _lib.DTYPES and all(params[i].dtype == dtype for i in which):
+        made = torch.empty(len(which) * dim, dtype=dtype, device=params[which[0]].device).split(dim)
+    else:
+        made = [torch.empty_like(params[i], dtype=params[i].dtype if params[i].dtype in _lib.DTYPES else torch.float32,
+                                 memory_format=torch.contiguous_format) for i in which]
+    to, types = a.d_param, a.d_param_dtype
+    for i, g in zip(which, made):
+        grads[i], to[i], types[i] = g, g.data_ptr(), _lib.DTYPES[g.dtype]
+    return grads
 
 
 class _Block(torch.autograd.Function):
@@ -207,8 +238,8 @@ class _Block(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, y, gate, scale, w1, b1, w2, b2, state, spec):
-        out, n, stats = _forward(spec, x, y, gate, scale, (w1, b1, w2, b2), True)
-        ctx.save_for_backward(x, y, gate, scale, w1, b1, w2, b2, state, stats)
+        out, n, ctx.call, ctx.stats = _forward(spec, x, y, gate, scale, (w1, b1, w2, b2), True)
+        ctx.save_for_backward(x, y, gate, scale, w1, b1, w2, b2, state)
         ctx.spec = spec
         ctx.set_materialize_grads(False)
         return (out, n) if out is not None and n is not None else (n if out is None else out)
@@ -216,51 +247,56 @@ class _Block(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        x, y, gate, scale, w1, b1, w2, b2, state, stats = ctx.saved_tensors
-        need, spec = ctx.needs_input_grad, ctx.spec
+        x, y, gate, scale, w1, b1, w2, b2, _ = ctx.saved_tensors
+        need, spec, (a, keep) = ctx.needs_input_grad, ctx.spec, ctx.call
         dout, dn = grads if len(grads) == 2 else ((None, grads[0]) if y is None else (grads[0], None))
         if dout is None and dn is None:
             return (None,) * 10
-        a, keep = _bind(spec, x, y, gate, scale, (w1, b1, w2, b2))
-        dim, dev, rows = a.dim, x.device, a.samples * a.tokens
+        if _still(a, x, y, gate, scale, (w1, b1, w2, b2)):
+            a = _lib.BlockArgs.from_buffer_copy(a)
+        else:
+            a, keep = _bind(spec, x, y, gate, scale, (w1, b1, w2, b2))
+        dim, rows = a.dim, a.samples * a.tokens
         # Without a gradient through the next norm dx is alpha dout: dout itself for 1.
         through = dn is None and spec.alpha == 1.0
-        dx = None if through or not (need[0] or dn is not None) else _empty(x, x.dtype)
-        dy = None if y is None else _empty(y, y.dtype)
-        dgate = None
+        dx = dy = dgate = None
+        if not through and (need[0] or dn is not None):
+            dx = _empty(x, x.dtype)
+            a.dx = dx.data_ptr()
+        if y is not None:
+            dy = _empty(y, y.dtype)
+            a.dy = dy.data_ptr()
         if gate is not None and (need[2] or spec.gate_kind != SAMPLE):
             dgate = _empty(gate, gate.dtype)
-        dparams = [None] * 5
-        for i, (t, at) in enumerate(((w1, 4), (b1, 5), (scale, 3), (w2, 6), (b2, 7))):
-            if t is not None and need[at]:
-                if not rows or (i >= 3 and dn is None):
-                    dparams[i] = torch.zeros_like(t)
-                    continue
-                g = torch.empty_like(t, dtype=t.dtype if t.dtype in _lib.DTYPES else torch.float32)
-                a.d_param[i], a.d_param_dtype[i] = g.data_ptr(), _lib.DTYPES[g.dtype]
-                dparams[i] = g if g.dtype == t.dtype else (g, t.dtype)
+            a.dgate = dgate.data_ptr()
+        params = (w1, b1, scale, w2, b2)
+        wanted = (need[4] and w1 is not None, need[5] and b1 is not None, need[3] and scale is not None,
+                  need[6] and w2 is not None, need[7] and b2 is not None)
         if rows:
+            after = dn is not None
+            dparams = _param_grads(a, params, wanted if after else (*wanted[:3], False, False), dim)
+            if not after and (wanted[3] or wanted[4]):
+                dparams = [torch.zeros_like(t) if w and g is None else g for g, t, w in zip(dparams, params, wanted)]
             a.splits, a.grid = _split(a.samples, a.tokens, dim, True)
             work = torch.empty((a.grid * 5 + (a.splits * a.samples if spec.gate_kind == SAMPLE else 0)) * dim,
-                               dtype=torch.float32, device=dev)
+                               dtype=torch.float32, device=x.device)
             if y is not None:
                 if dout is None:  # only n was used: a row of zeros, for every row
-                    dout = torch.zeros(1, dim, dtype=x.dtype, device=dev).expand(rows, dim)
+                    dout = torch.zeros(1, dim, dtype=x.dtype, device=x.device).expand(rows, dim)
                 dout, a.dout_stride = _rows(dout if dout.dtype == x.dtype else dout.to(x.dtype), dim)
-                a.dout, a.dy = dout.data_ptr(), dy.data_ptr()
-            if dn is not None:
+                a.dout = dout.data_ptr()
+            if after:
                 dn, a.dn_stride = _rows(dn if dn.dtype == spec.inner else dn.to(spec.inner), dim)
                 a.dn = dn.data_ptr()
-            if dx is not None:
-                a.dx = dx.data_ptr()
+            a.stats, a.work = ctx.stats.data_ptr(), work.data_ptr()
+            _lib.launch("p3d_block_bwd", x.device, a)
+        else:
+            dparams = [torch.zeros_like(t) if w else None for t, w in zip(params, wanted)]
             if dgate is not None:
-                a.dgate = dgate.data_ptr()
-            a.stats, a.work = stats.data_ptr(), work.data_ptr()
-            _lib.launch("p3d_block_bwd", dev, a)
-        elif dgate is not None:
-            dgate.zero_()
-        dw1, db1, dscale, dw2, db2 = (g[0].to(g[1]) if type(g) is tuple else g for g in dparams)
-        return (None if not need[0] else grads[0] if through else dx, dy if need[1] else None,
+                dgate.zero_()
+        dw1, db1, dscale, dw2, db2 = (g if g is None or g.dtype == t.dtype else g.to(t.dtype)
+                                      for g, t in zip(dparams, params))
+        return ((grads[0] if through else dx) if need[0] else None, dy if need[1] else None,
                 dgate if need[2] else None, dscale, dw1, db1, dw2, db2, None, None)
 
 
@@ -274,7 +310,7 @@ def _run(x, y, gate, scale, post, after, alpha, p, seed, inner):
         for t in (x, y, gate, scale, *params):
             if t is not None and t.requires_grad:
                 return _Block.apply(x, y, gate, scale, w1, b1, w2, b2, state, spec)
-    out, n, _ = _forward(spec, x, y, gate, scale, params, False)
+    out, n, _, _ = _forward(spec, x, y, gate, scale, params, False)
     return n if out is None else out if n is None else (out, n)
 
 

@@ -119,25 +119,26 @@ def _plan(tensors, positions, freqs, pairs, layout, magnitude):
 
 
 def _turn(plan, tensors, inverse):
-    """The tensors turned, each as a [B, H, N, d] view of a [B, N, H, d] buffer."""
-    first = tensors[0]
-    b, n, d = plan.batch, plan.tokens, plan.head_dim
-    heads = [t.shape[1] for t in tensors]
+    """The tensors turned, dense, with their dimensions in memory in the order of the inputs'."""
     outs, keep = [], []
     plan.inverse = inverse
-    for i, (t, h) in enumerate(zip(tensors, heads)):
+    for i, t in enumerate(tensors):
         s = t.stride()
         if s[3] != 1:
             t = t.contiguous()
             keep.append(t)
             s = t.stride()
-        out = torch.empty((b, n, h, d), dtype=first.dtype, device=first.device)
+        out = torch.empty_like(t)
+        o = out.stride()
+        if o[3] != 1:
+            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            o = out.stride()
         plan.x[i] = _lib.View(t.data_ptr(), s[0], s[1], s[2])
-        plan.y[i] = _lib.View(out.data_ptr(), n * h * d, d, h * d)
-        plan.heads[i] = h
-        outs.append(out.transpose(1, 2))
-    if first.numel():
-        _lib.launch("p3d_rotary", first.device, plan)
+        plan.y[i] = _lib.View(out.data_ptr(), o[0], o[1], o[2])
+        plan.heads[i] = t.shape[1]
+        outs.append(out)
+    if tensors[0].numel():
+        _lib.launch("p3d_rotary", tensors[0].device, plan)
     return tuple(outs)
 
 
@@ -163,7 +164,7 @@ def apply_rotary(tensors, positions, freqs, *, pairs=None, layout="interleaved",
     """Queries and keys turned to their positions: one tensor [batch, heads, tokens,
     head_dim] or a sequence of up to four alike but for their heads (any strides with
     contiguous channels, such as views of the projections); a tensor or a tuple comes
-    back, as transposed views of [batch, tokens, heads, head_dim] buffers.
+    back, dense, with tokens and heads in memory in the order of the input's.
 
     positions: int32 or int64 [tokens] or [batch, tokens]; for several axes of
     coordinates [..., tokens, axes] with ``pairs`` giving each axis its share of the
