@@ -296,14 +296,27 @@ def sum_rows(jobs, device):
     call("p3d_sum_rows", args, len(jobs), stream_of(device))
 
 
-def launch(name, device, *args):
-    """``call`` on the device's current stream, with that device current (a
-    launch goes to the current device, whatever stream it is given)."""
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return call(name, *args, stream_of(device))
-    if getattr(_lib or lib(), name)(*args, stream_of(device)) != 0:
-        raise RuntimeError(f"{name} failed: {lib().p3d_last_error().decode()}")
+_ops = None
+
+
+def ops():
+    """The host side of the operators around a block (binding/torch_ops.cpp), with the
+    entry points of the loaded library; raises if either has not been built."""
+    global _ops
+    if _ops is None:
+        handle = lib()
+        try:
+            from . import _torch_ops
+        except ImportError as e:
+            raise RuntimeError(f"pack3d_amd's torch binding does not load ({e}); build it with "
+                               "`python -m pack3d_amd.build`") from e
+        if _torch_ops.abi_version() != ABI_VERSION:
+            raise RuntimeError("pack3d_amd torch binding ABI mismatch; rebuild it")
+        _torch_ops.bind_library(*(ctypes.cast(getattr(handle, name), c_void_p).value for name in
+                                  ("p3d_block_fwd", "p3d_block_bwd", "p3d_dropout_apply", "p3d_rotary",
+                                   "p3d_last_error")))
+        _ops = _torch_ops
+    return _ops
 
 
 def require_device(t: torch.Tensor, what="tensor"):

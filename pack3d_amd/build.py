@@ -1,8 +1,9 @@
 """Build ``libpack3d_hip.so`` for gfx950 from ``pack3d_amd/csrc`` with hipcc.
 
 Usage: ``python -m pack3d_amd.build`` (or ``__graft_entry__.build()``).
-Objects go to ``pack3d_amd/_build``; the shared library lands next to this
-file so that it travels with the source tree.
+Objects go to ``pack3d_amd/_build``; the shared library and the torch binding
+(``_torch_ops.so``, the host side of the operators around a block) land next to
+this file so that they travel with the source tree.
 """
 from __future__ import annotations
 
@@ -18,6 +19,8 @@ PROBE_SRC = os.path.join(HERE, "probe")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libpack3d_hip.so")
 PROBE_LIB = os.path.join(HERE, "libpack3d_probe.so")
+BINDING_SRC = os.path.join(HERE, "binding", "torch_ops.cpp")
+BINDING = os.path.join(HERE, "_torch_ops.so")
 ARCH = "gfx950"
 
 # Packed fp32 VALU ops are disabled for device code: the compiler forms them
@@ -72,18 +75,43 @@ def _link(hipcc, objs, out, verbose):
         print(f"built {out}", flush=True)
 
 
+def _build_binding(hipcc, verbose):
+    """The host side of the operators around a block: a Python module on torch's C++ API."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               "/opt/rocm/include", sysconfig.get_paths()["include"]]
+    libs = os.path.join(root, "lib")
+    tmp = BINDING + ".tmp"
+    cmd = [hipcc, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_torch_ops",
+           *(flag for path in include for flag in ("-isystem", path)), BINDING_SRC, "-o", tmp, f"-L{libs}",
+           "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"compiling {BINDING_SRC} failed:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, BINDING)
+    if verbose:
+        print(f"built {BINDING}", flush=True)
+
+
 def build(verbose: bool = False) -> str:
     """Compile every HIP source and link the shared libraries: the product
-    library from csrc/, and the measurement library (the issue-rate probe of
-    probe/, with the status functions it reports through); returns the
-    product library's path."""
+    library from csrc/, the measurement library (the issue-rate probe of
+    probe/, with the status functions it reports through), and the torch
+    binding of binding/; returns the product library's path."""
     hipcc = _hipcc()
     os.makedirs(BUILD, exist_ok=True)
     sources = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
     probes = sorted(os.path.join(PROBE_SRC, f) for f in os.listdir(PROBE_SRC) if f.endswith(".hip"))
     workers = min(len(sources) + len(probes), int(os.environ.get("MAX_JOBS", "8")), 8)
     with concurrent.futures.ThreadPoolExecutor(max_workers=workers) as pool:
+        binding = pool.submit(_build_binding, hipcc, verbose)
         objs = list(pool.map(lambda s: _compile(s, hipcc, verbose), sources + probes))
+        binding.result()
     _link(hipcc, objs[:len(sources)], LIB, verbose)
     status = os.path.join(BUILD, "status.hip.o")
     _link(hipcc, objs[len(sources):] + [status], PROBE_LIB, verbose)

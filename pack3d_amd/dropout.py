@@ -10,7 +10,6 @@ of 2^-16; what is kept is divided by the share that this rate keeps.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -29,58 +28,29 @@ def new_seed(device):
 
 
 def mask_args(p, seed, device):
-    """The argument block of rate p and the tensor that it points into (or None).
-    seed: an int, a pair of ints (seed, offset), or an int64 tensor of these two on
-    the device, which the kernels read (no host synchronisation)."""
+    """(threshold, seed tensor or None, seed, offset) of rate p.  seed: an int, a pair of ints
+    (seed, offset), or an int64 tensor of these two on the device, which the kernels read
+    (no host synchronisation)."""
     threshold = threshold_of(p)
     if not threshold:
-        return _lib.Dropout(None, 0, 0, 0, 0), None
+        return 0, None, 0, 0
     if isinstance(seed, torch.Tensor):
         if seed.dtype != torch.int64 or seed.shape != (2,) or seed.device != device:
             raise ValueError("a seed tensor must be int64 [2] (seed, offset) on the input's device")
-        seed = seed if seed.stride(0) == 1 else seed.contiguous()
-        return _lib.Dropout(seed.data_ptr(), 0, 0, threshold, 0), seed
+        return threshold, seed if seed.stride(0) == 1 else seed.contiguous(), 0, 0
     pair = (seed, 0) if type(seed) is int else seed
     if not (isinstance(pair, (tuple, list)) and len(pair) == 2 and all(type(v) is int and 0 <= v < 2 ** 63
                                                                      for v in pair)):
         raise ValueError("dropout needs a seed: an int, a pair (seed, offset), both in [0, 2^63), or an int64 tensor [2]")
-    return _lib.Dropout(None, pair[0], pair[1], threshold, 0), None
-
-
-def _apply(x, mask):
-    x = x.contiguous()
-    y = torch.empty_like(x)
-    if x.numel():
-        _lib.launch("p3d_dropout_apply", x.device, x.data_ptr(), y.data_ptr(), x.numel(), _lib.DTYPES[x.dtype], mask)
-    return y
-
-
-class _CounterDropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, mask, state):
-        ctx.mask = mask
-        ctx.save_for_backward(state)
-        return _apply(x, mask)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        ctx.saved_tensors  # raises where the seed tensor was changed since the forward
-        return _apply(dy, ctx.mask), None, None
+    return threshold, None, *pair
 
 
 def counter_dropout(x, p, seed):
     """x with each element dropped at rate p (a multiple of 2^-16, the nearest) and the
     others divided by 1 - p.  The same seed gives the same mask, in the backward too;
     another call needs another seed or offset.  fp32, fp16 and bf16, any shape (a
-    tensor that is not contiguous is copied first)."""
-    if not x.is_cuda:
-        _lib.require_device(x, "x")
-    if x.dtype not in _lib.DTYPES:
-        raise ValueError("counter_dropout takes fp32, fp16 or bf16")
-    mask, state = mask_args(p, seed, x.device)
-    if not mask.threshold:
+    tensor that is not contiguous is copied first); differentiable (first order)."""
+    mask = mask_args(p, seed, x.device)
+    if not mask[0] and x.is_cuda and x.dtype in _lib.DTYPES:
         return x
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _CounterDropout.apply(x, mask, state)
-    return _apply(x, mask)
+    return _lib.ops().dropout(x, *mask)

@@ -14,14 +14,12 @@ import math
 from dataclasses import dataclass
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .rope import _cached
 
 LAYOUTS = ("interleaved", "half")
 SCALINGS = ("none", "linear", "ntk", "parts")
-MAX_TENSORS = 4
 
 
 def rotary_frequencies(pairs, *, base=10000.0, scaling="none", factor=1.0, trained=None, fast=32.0, slow=1.0):
@@ -59,107 +57,6 @@ def rotary_frequencies(pairs, *, base=10000.0, scaling="none", factor=1.0, train
     return torch.cat(made), magnitude
 
 
-def _plan(tensors, positions, freqs, pairs, layout, magnitude):
-    """Checks of apply_rotary's arguments; the argument block without the tensors, and
-    the frequencies as it points at them."""
-    if not 1 <= len(tensors) <= MAX_TENSORS:
-        raise ValueError("apply_rotary takes one to four tensors")
-    first = tensors[0]
-    shape, dtype, device = first.shape, first.dtype, first.device
-    if len(shape) != 4:
-        raise ValueError("tensors must be [batch, heads, tokens, head_dim]")
-    b, _, n, d = shape
-    for t in tensors:
-        if t.dtype != dtype or t.device != device or t.shape != (b, t.shape[1], n, d):
-            raise ValueError("tensors must be [batch, heads, tokens, head_dim] of one type, alike but for the heads")
-        if not 0 < t.shape[1] * (d // 8 + 2) <= 8192:
-            raise ValueError("heads must be at least 1, heads * (head_dim / 8 + 2) at most 8192")
-    if not first.is_cuda:
-        _lib.require_device(first, "q and k")
-    if dtype not in _lib.DTYPES:
-        raise ValueError("apply_rotary takes fp32, fp16 or bf16")
-    if freqs.dtype != torch.float64 or freqs.ndim != 1 or freqs.device != device:
-        raise ValueError("freqs must be float64 [pairs] on the tensors' device (rotary_frequencies)")
-    count = freqs.shape[0]
-    if not 1 <= count <= d // 2 or d > 1024:
-        raise ValueError("freqs must have 1 to head_dim / 2 pairs, head_dim at most 1024")
-    a = _lib.RotaryArgs()
-    axes = 1
-    if pairs is None:
-        a.axis_pairs[0] = count
-    else:
-        axes = len(pairs)
-        if not 1 <= axes <= 3 or sum(pairs) != count:
-            raise ValueError("pairs must give each of one to three axes its count of freqs")
-        for i, c in enumerate(pairs):
-            if type(c) is not int or c < 0:
-                raise ValueError("pairs must be counts")
-            a.axis_pairs[i] = c
-    if layout not in LAYOUTS:
-        raise ValueError("layout must be interleaved or half")
-    if not math.isfinite(magnitude):
-        raise ValueError("magnitude must be finite")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.device != device:
-        raise ValueError("positions must be int32 or int64 on the tensors' device")
-    of, strides = positions.shape, positions.stride()
-    if axes == 1:
-        of, strides = (*of, 1), (*strides, 1)
-    if len(of) == 2:
-        of, strides = (1, *of), (0, *strides)
-    if len(of) != 3 or of[0] not in (1, b) or of[1:] != (n, axes):
-        raise ValueError("positions must be [tokens] or [batch, tokens], with an axis dimension last for several axes")
-    a.tokens, a.count, a.batch, a.head_dim, a.pairs, a.axes = n, len(tensors), b, d, count, axes
-    a.positions = positions.data_ptr()
-    a.pos_sb, a.pos_sn, a.pos_sa = 0 if of[0] == 1 else strides[0], strides[1], strides[2]
-    freqs = freqs.contiguous()
-    a.freqs = freqs.data_ptr()
-    a.pos_is64, a.half, a.dtype = positions.dtype == torch.int64, layout == "half", _lib.DTYPES[dtype]
-    a.magnitude = magnitude
-    return a, freqs
-
-
-def _turn(plan, tensors, inverse):
-    """The tensors turned, dense, with their dimensions in memory in the order of the inputs'."""
-    outs, keep = [], []
-    plan.inverse = inverse
-    for i, t in enumerate(tensors):
-        s = t.stride()
-        if s[3] != 1:
-            t = t.contiguous()
-            keep.append(t)
-            s = t.stride()
-        out = torch.empty_like(t)
-        o = out.stride()
-        if o[3] != 1:
-            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-            o = out.stride()
-        plan.x[i] = _lib.View(t.data_ptr(), s[0], s[1], s[2])
-        plan.y[i] = _lib.View(out.data_ptr(), o[0], o[1], o[2])
-        plan.heads[i] = t.shape[1]
-        outs.append(out)
-    if tensors[0].numel():
-        _lib.launch("p3d_rotary", tensors[0].device, plan)
-    return tuple(outs)
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, plan, positions, freqs, *tensors):
-        ctx.plan = plan
-        ctx.save_for_backward(positions, freqs)
-        return _turn(plan, tensors, 0)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
-        ctx.saved_tensors  # raises where positions or freqs were changed since the forward
-        need = [i for i in range(len(grads)) if ctx.needs_input_grad[3 + i]]
-        plan = _lib.RotaryArgs.from_buffer_copy(ctx.plan)
-        plan.count = len(need)
-        back = dict(zip(need, _turn(plan, [grads[i] for i in need], 1)))
-        return (None, None, None, *(back.get(i) for i in range(len(grads))))
-
-
 def apply_rotary(tensors, positions, freqs, *, pairs=None, layout="interleaved", magnitude=1.0):
     """Queries and keys turned to their positions: one tensor [batch, heads, tokens,
     head_dim] or a sequence of up to four alike but for their heads (any strides with
@@ -172,14 +69,11 @@ def apply_rotary(tensors, positions, freqs, *, pairs=None, layout="interleaved",
     head turn, channels 2j and 2j + 1 (interleaved) or j and P + j (half), and are
     multiplied by magnitude; the rest are copied.  Angles are formed in 64 bits.
     Differentiable in the tensors (first order)."""
+    if layout not in LAYOUTS:
+        raise ValueError("layout must be interleaved or half")
     one = isinstance(tensors, torch.Tensor)
-    tensors = (tensors,) if one else tuple(tensors)
-    plan, freqs = _plan(tensors, positions, freqs, pairs, layout, float(magnitude))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        outs = _Rotary.apply(plan, positions, freqs, *tensors)
-    else:
-        outs = _turn(plan, tensors, 0)
-    return outs[0] if one else outs
+    outs = _lib.ops().rotary([tensors] if one else tensors, positions, freqs, pairs, layout == "half", magnitude)
+    return outs[0] if one else tuple(outs)
 
 
 @dataclass(frozen=True)

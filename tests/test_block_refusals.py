@@ -6,7 +6,6 @@ import torch
 
 import pack3d_amd as p3d
 from pack3d_amd import _lib
-from pack3d_amd.block import _split
 from pack3d_amd.dropout import mask_args, threshold_of
 
 
@@ -148,5 +147,5 @@ def test_encoding_refusals(kw):
 @pytest.mark.parametrize("dim", [1, 64, 192, 512, 513, 8192])
 @pytest.mark.parametrize("backward", [False, True])
 def test_splits_stay_within_what_the_kernels_take(samples, tokens, dim, backward):
-    splits, grid = _split(samples, tokens, dim, backward)
+    splits, grid = _lib.ops().block_split(samples, tokens, dim, backward)
     assert 1 <= splits <= tokens and 1 <= grid <= splits * samples and splits * samples < 2 ** 31

@@ -325,3 +325,81 @@ def test_inputs_changed_before_the_backward_raise(gpu):
     seed.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         torch.autograd.grad(out.sum(), x)
+
+
+def _ways(gpu):
+    """One call of each operator on a leaf x: name -> (leaf, function of it)."""
+    freqs = p3d.rotary_frequencies(8)[0].to(gpu)
+    positions = torch.arange(6, device=gpu)
+    w = torch.ones(24, device=gpu, requires_grad=True)
+    gate = torch.full((2, 1, 24), 0.5, device=gpu)
+
+    def leaf(*shape):
+        return torch.randn(*shape, device=gpu, requires_grad=True)
+    return {"residual": (leaf(2, 5, 24), lambda x: p3d.block_residual(x, x.detach() * 2, post_norm=p3d.Norm("rms", w), gate=gate,
+                                                                       p=0.3, seed=4, next_norm=p3d.Norm("layer", w))[1]),
+            "norm": (leaf(7, 24), lambda x: p3d.block_norm(x, p3d.Norm("layer", w))),
+            "dropout": (leaf(7, 24), lambda x: p3d.counter_dropout(x, 0.3, 4)),
+            "rotary": (leaf(2, 3, 6, 16), lambda x: p3d.apply_rotary(x, positions, freqs))}
+
+
+@pytest.mark.parametrize("name", ["residual", "norm", "dropout", "rotary"])
+def test_autograd_contract(gpu, name):
+    """A graph kept and gone, saved tensors that come back as others, second order and forward mode refused."""
+    x, f = _ways(gpu)[name]
+    up = torch.randn_like(f(x))
+    (g,) = torch.autograd.grad(f(x), x, up)
+    out = f(x)
+    assert torch.equal(torch.autograd.grad(out, x, up, retain_graph=True)[0], g)
+    assert torch.equal(torch.autograd.grad(out, x, up)[0], g)
+    if name in ("residual", "norm", "rotary"):
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(out, x, up)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(gpu)):
+        moved = f(x)
+    assert torch.equal(torch.autograd.grad(moved, x, up)[0], g)
+    again = up.clone().requires_grad_()
+    (first,) = torch.autograd.grad(f(x), x, again, create_graph=True)
+    assert torch.equal(first.detach(), g) and first.requires_grad
+    for by in (again, x) if name in ("residual", "norm") else (again,):  # the others are linear in x
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            torch.autograd.grad(first.sum(), by, retain_graph=True)
+    import torch.autograd.forward_ad as fwad
+    with fwad.dual_level():
+        dual = fwad.make_dual(x.detach(), torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            f(dual)
+    x.grad = None
+    f(x).backward(up)
+    f(x).backward(up)
+    assert torch.allclose(x.grad, 2 * g)
+
+
+def test_calls_from_two_threads(gpu):
+    """Each thread on a stream of its own, forward and backward, against the same calls made alone."""
+    import threading
+    shapes = [(2, 300, 192), (1, 700, 327)]
+
+    def work(shape, seed):
+        gen = torch.Generator(device=gpu).manual_seed(seed)
+        x, y, up = (torch.randn(shape, generator=gen, device=gpu) for _ in range(3))
+        x, y = x.requires_grad_(), y.requires_grad_()
+        out, n = p3d.block_residual(x, y, post_norm=p3d.Norm("rms"), p=0.2, seed=seed, next_norm=p3d.Norm("layer"))
+        return [out.detach(), n.detach(), *torch.autograd.grad((out, n), (x, y), (up, up))]
+    alone = [work(s, i) for i, s in enumerate(shapes)]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i] = work(shapes[i], i)
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(alone, got):
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
