@@ -109,7 +109,7 @@ constexpr int64_t kMaxStride = 1LL << 29;  // elements between rows
 
 // Ranges that a sample's rows are cut into, and workgroups.
 std::pair<int64_t, int64_t> block_split(int64_t samples, int64_t tokens, int64_t dim, bool backward) {
-    int64_t threads = 8;  // of a row
+    int64_t threads = dim < 4 ? 4 : 2;  // of a row
     while (threads < 512 && dim > threads * 8) threads *= 2;
     const int64_t rows = threads <= 64 ? 256 / threads : 1;  // that a workgroup holds at a time
     const int64_t per_sample = (tokens + rows - 1) / rows, steps = per_sample * samples;

@@ -248,7 +248,8 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_fwd(BlockDev a) {
                     }
                 }
                 if (mask.threshold) {
-                    const uint32_t bits = keep_run<TPR, E>(mask, row, a.dim, c, at.sub);
+                    uint32_t bits = 0;
+                    if (TPR <= 64 || at.in_row()) bits = keep_run<TPR, E>(mask, row, a.dim, c, at.sub);
 #pragma unroll
                     for (int e = 0; e < E; ++e) z[e] = and_word(z[e], bit_word(bits, e));
                 }
@@ -290,7 +291,7 @@ template <typename TX, typename TY, int TPR, int E, int FORM, bool NEXT>
 __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
     constexpr int GROUPS = TPR > 64 ? 1 : 256 / TPR;
     constexpr bool HAS_Y = FORM != kNorm, GATED = FORM == kEndGated;
-    __shared__ float lds[TPR > 64 ? RowSum<TPR>::LDS : 256 * E];
+    __shared__ float lds[TPR > 64 ? RowSum<TPR>::LDS : 4 * TPR * E];
     RowSum<TPR> row_sum{lds};
     const Place<TPR, E> at(a.dim);
     const int c = at.c;
@@ -315,18 +316,24 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) dw1[e] = db1[e] = dsc[e] = dw2[e] = db2[e] = 0.f;
 
-    // Sum over the workgroup's row groups, in order; group 0 ends with it and stores it.
+    // Sum over the workgroup's row groups, in a fixed order; group 0 stores it.
     auto gather = [&](float(&v)[E], float* to) {
         if constexpr (GROUPS > 1) {
-            __syncthreads();
+            // The groups of a wave by lanes, then the four waves in order.
 #pragma unroll
-            for (int e = 0; e < E; ++e) lds[e * 256 + threadIdx.x] = v[e];
-            __syncthreads();
-            if (at.grp == 0) {
+            for (int o = TPR; o < 64; o *= 2)
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    for (int k = 1; k < GROUPS; ++k) v[e] += lds[e * 256 + k * TPR + at.sub];
+                for (int e = 0; e < E; ++e) v[e] += __shfl_xor(v[e], o);
+            __syncthreads();
+            if ((threadIdx.x & 63) < TPR) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) lds[((threadIdx.x >> 6) * E + e) * TPR + at.sub] = v[e];
             }
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                v[e] = (lds[e * TPR + at.sub] + lds[(E + e) * TPR + at.sub]) +
+                       (lds[(2 * E + e) * TPR + at.sub] + lds[(3 * E + e) * TPR + at.sub]);
         }
         if (at.grp == 0 && at.in_row()) {
             Run<float, E> o;
@@ -556,23 +563,32 @@ int launch_as(const BlockDev& a, bool backward, unsigned grid, hipStream_t s) {
 
 }  // namespace
 
-// Threads of a row and channels a thread: eight channels (16 bytes of a 16-bit type),
-// with the fewest threads, a power of two, that cover the row; six where they fill
-// the lanes better (96, 192 and 384 channels: 3/4 of the lanes hold eight).
+// Threads of a row and channels a thread: eight channels (16 bytes of a 16-bit type)
+// over the fewest threads, a power of two, that cover the row; six where those cover it
+// too (160 channels: 27 lanes of 32 hold six, 20 hold eight; 200,000 rows forward and
+// backward 160 against 169 us).  Rows of 3, 5 or 7 waves fill fewer of a CU's wave slots:
+// 25,000 rows of 1,280 took 215 us in three waves, 170 in four of which two have no
+// channels.  block_split in binding/torch_ops.cpp deals out rows by the same widths.
 template <typename TX, typename TY>
 int launch_block(const BlockDev& a, bool backward, unsigned grid, hipStream_t s) {
     const int d = a.dim;
-    if (d < 8) return launch_as<TX, TY, 8, 1>(a, backward, grid, s);
+    if (d < 4) return launch_as<TX, TY, 4, 1>(a, backward, grid, s);
+    if (d < 8) return launch_as<TX, TY, 2, 4>(a, backward, grid, s);
+    if (d <= 16) return launch_as<TX, TY, 2, 8>(a, backward, grid, s);
+    if (d <= 32) return launch_as<TX, TY, 4, 8>(a, backward, grid, s);
     if (d <= 64) return launch_as<TX, TY, 8, 8>(a, backward, grid, s);
-    if (d <= 96 && d % 6 == 0) return launch_as<TX, TY, 16, 6>(a, backward, grid, s);
+    if (d <= 96) return launch_as<TX, TY, 16, 6>(a, backward, grid, s);
     if (d <= 128) return launch_as<TX, TY, 16, 8>(a, backward, grid, s);
-    if (d <= 192 && d % 6 == 0) return launch_as<TX, TY, 32, 6>(a, backward, grid, s);
+    if (d <= 192) return launch_as<TX, TY, 32, 6>(a, backward, grid, s);
     if (d <= 256) return launch_as<TX, TY, 32, 8>(a, backward, grid, s);
-    if (d <= 384 && d % 6 == 0) return launch_as<TX, TY, 64, 6>(a, backward, grid, s);
+    if (d <= 384) return launch_as<TX, TY, 64, 6>(a, backward, grid, s);
     if (d <= 512) return launch_as<TX, TY, 64, 8>(a, backward, grid, s);
-    if (d <= 1024) return launch_as<TX, TY, 128, 8>(a, backward, grid, s);
-    if (d <= 2048) return launch_as<TX, TY, 256, 8>(a, backward, grid, s);
-    if (d <= 4096) return launch_as<TX, TY, 512, 8>(a, backward, grid, s);
+    if (d <= 128 * 6) return launch_as<TX, TY, 128, 6>(a, backward, grid, s);
+    if (d <= 128 * 8) return launch_as<TX, TY, 128, 8>(a, backward, grid, s);
+    if (d <= 256 * 6) return launch_as<TX, TY, 256, 6>(a, backward, grid, s);
+    if (d <= 256 * 8) return launch_as<TX, TY, 256, 8>(a, backward, grid, s);
+    if (d <= 512 * 6) return launch_as<TX, TY, 512, 6>(a, backward, grid, s);
+    if (d <= 512 * 8) return launch_as<TX, TY, 512, 8>(a, backward, grid, s);
     return launch_as<TX, TY, 512, 16>(a, backward, grid, s);
 }
 

@@ -40,8 +40,8 @@ __device__ __forceinline__ char* row_address(char* base, uint32_t row, uint32_t 
     return base + (uint64_t)row * stride;
 }
 
-// Sum over an aligned group of LANES lanes (a power of two up to 64); every lane of the
-// group ends with the same bits.
+// Sum over an aligned group of LANES lanes (a power of two from 2 to 64); every lane of
+// the group ends with the same bits.
 template <int LANES>
 __device__ __forceinline__ float group_sum(float x) {
     x += dpp_move<0xB1>(x);
@@ -67,7 +67,9 @@ __device__ __forceinline__ float group_sum(float x) {
 template <int TPR>
 struct RowSum {
     static constexpr int WAVES = TPR > 64 ? TPR / 64 : 1;
-    static constexpr int LDS = TPR > 64 ? 2 * WAVES * 3 : 1;
+    // Lanes that add the waves' sums: the next power of two, the last ones adding nothing.
+    static constexpr int SLOTS = WAVES <= 2 ? 2 : (WAVES <= 4 ? 4 : (WAVES <= 8 ? 8 : 16));
+    static constexpr int LDS = TPR > 64 ? 2 * SLOTS * 3 : 1;
     float* lds;  // LDS floats
     int turn = 0;
 
@@ -77,15 +79,19 @@ struct RowSum {
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = group_sum<(TPR > 64 ? 64 : TPR)>(x[i]);
         if constexpr (TPR > 64) {
-            float* buf = lds + turn * WAVES * 3;
+            float* buf = lds + turn * SLOTS * 3;
             turn ^= 1;
             if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) buf[i * WAVES + (threadIdx.x >> 6)] = x[i];
+                for (int i = 0; i < N; ++i) buf[i * SLOTS + (threadIdx.x >> 6)] = x[i];
             }
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = group_sum<WAVES>(buf[i * WAVES + threadIdx.x % WAVES]);
+            for (int i = 0; i < N; ++i) {
+                const int slot = threadIdx.x % SLOTS;
+                const float s = buf[i * SLOTS + slot];
+                x[i] = group_sum<SLOTS>(SLOTS == WAVES || slot < WAVES ? s : 0.f);
+            }
         }
     }
 };

@@ -112,11 +112,13 @@ def test_residual_kinds(gpu, outer, inner, post, after, gate, scale, alpha, p):
     _run_case(gpu, post, after, alpha, p, 3, 37, 72, outer, inner, gate, scale)
 
 
-@pytest.mark.parametrize("dim", [1, 2, 7, 8, 9, 63, 64, 65, 128, 131, 192, 256, 327, 512, 513, 1000, 1024, 1500, 2048, 2049,
-                                 4096, 5001, 8191, 8192])
+@pytest.mark.parametrize("dim", [1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 24, 32, 33, 63, 64, 65, 96, 97, 128, 131, 160, 192, 200, 256, 264, 327,
+                                 384, 385, 512, 513, 520, 768, 769, 1000, 1024, 1025, 1500, 1536, 1537, 2048, 2049, 2560, 2561, 3001, 3584,
+                                 3585, 4096, 4097, 5001, 8191, 8192])
 def test_residual_widths(gpu, dim):
     print(f"block_residual dim {dim}", flush=True)
     _run_case(gpu, "layer", "rms", 1.25, 0.1, 2, 5, dim, F32, BF16, "sample", True)
+    _run_case(gpu, "layer", "layer", 1.0, 0.3, 1, 70, dim, F32, F32, "full", True)
     _run_case(gpu, "rms", "layer", 1.0, 0.2, 1, 3, dim, F16, F16, "token", True)
 
 
