@@ -110,16 +110,16 @@ constexpr int64_t kMaxStride = 1LL << 29;  // elements between rows
 // Ranges that a sample's rows are cut into, and workgroups.
 std::pair<int64_t, int64_t> block_split(int64_t samples, int64_t tokens, int64_t dim, bool backward) {
     int64_t threads = dim < 4 ? 4 : 2;  // of a row
-    while (threads < 512 && dim > threads * 8) threads *= 2;
+    while (threads < 1024 && dim > threads * 8) threads *= 2;
     const int64_t rows = threads <= 64 ? 256 / threads : 1;  // that a workgroup holds at a time
     const int64_t per_sample = (tokens + rows - 1) / rows, steps = per_sample * samples;
     int64_t wanted;
     if (backward) {
         // One round of what the GPU runs at a time (two waves a SIMD): each workgroup
         // leaves a row of partial parameter gradients.
-        wanted = (1 << 17) / (threads > 64 ? threads : 256);
+        wanted = std::max<int64_t>(256, (1 << 17) / (threads > 64 ? threads : 256));
     } else if (threads > 64) {
-        wanted = (1 << 18) / threads;
+        wanted = std::max<int64_t>(512, (1 << 18) / threads);
     } else {
         // Several rounds, of at least four steps each once every CU has work: a workgroup
         // begins by loading the parameters (4,913 x 3 rows of 327: 21 us in 921, 25 in 3,685).

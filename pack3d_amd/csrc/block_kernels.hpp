@@ -19,7 +19,7 @@
 // TPR threads share a row and hold E consecutive channels each, so a row is read
 // once into registers whatever its width.  Rows of up to 512 channels lie within a
 // wave, several to a wave below that; wider ones take a workgroup.  The next row's
-// loads are issued before the present one is worked on.
+// loads are issued before the present one is worked on (where registers allow).
 //
 // Where E does not divide the width, the row's last lane holds its last E channels
 // and shares some with its neighbour: both compute and store the same bits, and sums
@@ -291,6 +291,9 @@ template <typename TX, typename TY, int TPR, int E, int FORM, bool NEXT>
 __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
     constexpr int GROUPS = TPR > 64 ? 1 : 256 / TPR;
     constexpr bool HAS_Y = FORM != kNorm, GATED = FORM == kEndGated;
+    // Rows of 1,024 threads leave 128 registers a thread: the next row's loads would be
+    // spilled (5,333 rows of 6,144 forward and backward 255 us with, 173 without).
+    constexpr bool AHEAD = TPR <= 512 || FORM == kNorm;
     __shared__ float lds[TPR > 64 ? RowSum<TPR>::LDS : 4 * TPR * E];
     RowSum<TPR> row_sum{lds};
     const Place<TPR, E> at(a.dim);
@@ -382,9 +385,10 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
                 }
             };
             const int last = unit.count - 1;
-            fetch(unit.first + min(at.grp, last));
+            if constexpr (AHEAD) fetch(unit.first + min(at.grp, last));
             for (int i = at.grp; i <= last; i += GROUPS) {
                 const uint32_t row = unit.first + i;
+                if constexpr (!AHEAD) fetch(row);
                 float go[E], xh2[E], g2[E], xh1[E], g[E];
                 if constexpr (HAS_Y) {
                     yr.to(xh1);
@@ -399,7 +403,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
                 }
                 if constexpr (GATED) gr.to(a, g);
                 const float mean1 = st[0], rstd1 = st[1], mean2 = st[2], rstd2 = st[3];
-                fetch(unit.first + min(i + GROUPS, last));
+                if constexpr (AHEAD) fetch(unit.first + min(i + GROUPS, last));
                 uint32_t bits = 0xffffffffu;
                 float b[E];  // keep b, and times the gate where it has one a token
                 if constexpr (HAS_Y) {
@@ -589,7 +593,8 @@ int launch_block(const BlockDev& a, bool backward, unsigned grid, hipStream_t s)
     if (d <= 256 * 8) return launch_as<TX, TY, 256, 8>(a, backward, grid, s);
     if (d <= 512 * 6) return launch_as<TX, TY, 512, 6>(a, backward, grid, s);
     if (d <= 512 * 8) return launch_as<TX, TY, 512, 8>(a, backward, grid, s);
-    return launch_as<TX, TY, 512, 16>(a, backward, grid, s);
+    if (d <= 1024 * 6) return launch_as<TX, TY, 1024, 6>(a, backward, grid, s);
+    return launch_as<TX, TY, 1024, 8>(a, backward, grid, s);
 }
 
 }  // namespace p3d

@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t keep_group(const MaskDev& m, uint64_t group)
     return bits;
 }
 
-// Bits of a lane's E elements (at most 8 within a wave, 16 beyond), from channel c of row `row` on, in a tensor of rows
+// Bits of a lane's E <= 8 elements, from channel c of row `row` on, in a tensor of rows
 // of dim.  TPR lanes (every one of them here) hold the row, lane `sub` of them from
 // channel E sub on or less.
 //
@@ -89,9 +89,7 @@ __device__ __forceinline__ uint32_t keep_run(const MaskDev& m, uint32_t row, int
         const uint64_t first = start + c;
         const uint32_t shift = (uint32_t)first & 7;
         uint32_t bits = keep_group(m, first >> 3);
-#pragma unroll
-        for (int k = 1; k < (E + 14) / 8; ++k)
-            if (shift + E > 8 * k) bits |= keep_group(m, (first >> 3) + k) << (8 * k);
+        if (shift + E > 8) bits |= keep_group(m, (first >> 3) + 1) << 8;
         return bits >> shift;
     } else {
         const uint64_t group = start >> 3;
