@@ -37,6 +37,7 @@ struct RotaryDev {
     int run;                            // tokens of a tile
     int head_dim, pairs;
     uint32_t chunks, turned, chunks_inv;  // steps of a head, of which `turned` hold pairs
+    int full, copied;                   // pairs of a step (8, or all of fewer); first channel of the steps that copy
     const void* positions;
     int64_t pb, pn, pa;                 // strides of the positions
     int pos64, end0, end1;              // pairs below end0 are on axis 0, below end1 on axis 1
@@ -47,9 +48,12 @@ struct RotaryDev {
 // a / d for a < 2^32 / d, with inv = ceil(2^32 / d); d = 1 has inv = 0.
 __device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t inv) { return inv ? __umulhi(a, inv) : a; }
 
-// One step: sixteen channels that turn (two runs of eight, apart or adjacent), or eight
-// that are copied.  SMALL: heads with fewer than eight pairs, or with one to seven
-// channels to copy, whose runs are shorter than eight.
+// One step: eight pairs (two runs of eight channels, apart or adjacent), or eight channels
+// that are copied.  Heads with fewer than eight pairs have one step of them, which reads
+// runs of eight all the same: adjacent, it copies the channels behind the pairs too; apart,
+// it stores what is the pairs' (30M bf16 channels in heads of 16 with 3 pairs: 26 and 60
+// us; whole heads 27).  Copies of fewer than eight channels read the head's last eight and
+// store what is theirs.  SMALL: heads of fewer than 16 channels, an element at a time.
 template <typename T, bool HALF, bool SMALL>
 struct Step {
     const char* src;
@@ -63,18 +67,18 @@ struct Step {
         const uint32_t t = quotient(i, a.steps_inv[k]), r = i - t * a.steps[k];
         const uint32_t h = quotient(r, a.chunks_inv), c = r - h * a.chunks;
         const p3d_view &x = a.x[k], &y = a.y[k];
-        const int P = a.pairs, left = a.head_dim - 2 * P;
+        const int P = a.pairs;
         int64_t channel;
         if (c < a.turned) {
-            const int j = SMALL ? (int)c * kPiece : min((int)c * kPiece, P - kPiece);
+            const int j = SMALL ? (int)c * kPiece : min((int)c * kPiece, P - a.full);
             at = t * P + j;
-            count = SMALL ? min(kPiece, P - j) : kPiece;
+            count = SMALL ? min(kPiece, P - j) : a.full;
             channel = HALF ? j : 2 * j;
         } else {
-            const int j = (int)(c - a.turned) * kPiece;
+            const int j = a.copied + (int)(c - a.turned) * kPiece;
             at = 0;
-            count = -min(kPiece, left - j);
-            channel = SMALL ? 2 * P + j : min(2 * P + j, a.head_dim - kPiece);
+            count = -min(kPiece, a.head_dim - j);
+            channel = SMALL ? j : min(j, a.head_dim - kPiece);
         }
         src = reinterpret_cast<const char*>(reinterpret_cast<const T*>(x.data) + b * x.sb + (int64_t)h * x.sh +
                                             (first + t) * x.sn + channel);
@@ -114,12 +118,13 @@ struct Step {
             v.to(g);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) {
-                const float2 w = table[at + (SMALL && e >= count ? 0 : e)];
+                const bool real = SMALL ? e < count : e < a.full;
+                const float2 w = table[at + (real ? e : 0)];
                 float& p = HALF ? f[e] : (e < kPiece / 2 ? f[(2 * e) % kPiece] : g[(2 * e) % kPiece]);
                 float& q = HALF ? g[e] : (e < kPiece / 2 ? f[(2 * e + 1) % kPiece] : g[(2 * e + 1) % kPiece]);
                 const float s = p * w.x - q * w.y, t = p * w.y + q * w.x;
-                p = s;
-                q = t;
+                p = real ? s : p;
+                q = real ? t : q;
             }
             u.from(f);
             v.from(g);
@@ -128,7 +133,10 @@ struct Step {
             store_some(u, dst, first_run());
             store_some(v, dst + apart(a), second_run());
         } else {
-            if (count == -kPiece || count > 0) {
+            if (count > 0 && HALF && a.full < kPiece) {
+                store_some(u, dst, a.full);
+                store_some(v, dst + apart(a), a.full);
+            } else if (count == -kPiece || count > 0) {
                 u.store(dst);
                 if (count > 0) v.store(dst + apart(a));
             } else {
@@ -213,9 +221,11 @@ extern "C" int p3d_rotary(const p3d_rotary_args* args, void* stream) {
     a.tokens = g.tokens;
     a.head_dim = g.head_dim;
     a.pairs = g.pairs;
-    const int left = g.head_dim - 2 * g.pairs;
     a.turned = (uint32_t)cdiv(g.pairs, kPiece);
-    a.chunks = a.turned + (uint32_t)cdiv(left, kPiece);
+    const bool small = g.head_dim < 2 * kPiece;
+    a.full = g.pairs < kPiece ? g.pairs : kPiece;
+    a.copied = !small && !g.half && g.pairs < kPiece ? 2 * kPiece : 2 * g.pairs;
+    a.chunks = a.turned + (uint32_t)cdiv(g.head_dim - a.copied, kPiece);
     a.chunks_inv = inverse_of(a.chunks);
     a.count = g.count;
     uint32_t most = 0;
@@ -248,7 +258,6 @@ extern "C" int p3d_rotary(const p3d_rotary_args* args, void* stream) {
     P3D_REQUIRE(g.batch * cdiv(g.tokens, run) < (1LL << 31), "launch grid too large");
     a.tiles = (uint32_t)cdiv(g.tokens, run);
     const unsigned blocks = (unsigned)g.batch * a.tiles;
-    const bool small = g.pairs < kPiece;
     hipStream_t s = as_stream(stream);
     switch (g.dtype) {
         case P3D_F32: launch<float>(a, g.half, small, blocks, s); break;

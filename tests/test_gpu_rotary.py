@@ -53,7 +53,8 @@ def _run(gpu, b, heads, n, d, pairs, layout, dtype, positions, magnitude=1.0, sc
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("layout", ["interleaved", "half"])
 @pytest.mark.parametrize("d,pairs", [(16, 8), (16, 3), (48, 24), (64, 32), (64, 16), (80, 37), (128, 64), (128, 1),
-                                     (2, 1), (7, 3), (33, 13), (256, 128), (1024, 512)])
+                                     (2, 1), (7, 3), (15, 7), (16, 7), (17, 1), (24, 5), (20, 8), (40, 4),
+                                     (33, 13), (256, 128), (1024, 512)])
 def test_heads_and_layouts(gpu, dtype, layout, d, pairs):
     _run(gpu, 2, (4, 2), 29, d, (pairs,), layout, dtype, torch.arange(29) * 3)
 
