@@ -37,7 +37,7 @@ struct RotaryDev {
     int run;                            // tokens of a tile
     int head_dim, pairs;
     uint32_t chunks, turned, chunks_inv;  // steps of a head, of which `turned` hold pairs
-    int full, copied;                   // pairs of a step (8, or all of fewer); first channel of the steps that copy
+    int copied;                         // first channel of the steps that copy
     const void* positions;
     int64_t pb, pn, pa;                 // strides of the positions
     int pos64, end0, end1;              // pairs below end0 are on axis 0, below end1 on axis 1
@@ -53,9 +53,12 @@ __device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t inv) { return 
 // runs of eight all the same: adjacent, it copies the channels behind the pairs too; apart,
 // it stores what is the pairs' (30M bf16 channels in heads of 16 with 3 pairs: 26 and 60
 // us; whole heads 27).  Copies of fewer than eight channels read the head's last eight and
-// store what is theirs.  SMALL: heads of fewer than 16 channels, an element at a time.
-template <typename T, bool HALF, bool SMALL>
+// store what is theirs.  Heads of fewer than 16 channels go an element at a time.
+enum Form { kWhole, kFew, kSmall };  // eight pairs or more; fewer; heads of fewer than 16 channels
+
+template <typename T, bool HALF, int FORM>
 struct Step {
+    static constexpr bool FEW = FORM == kFew, SMALL = FORM == kSmall;
     const char* src;
     char* dst;
     uint32_t at;  // of the (cos, sin) of its first pair
@@ -70,9 +73,9 @@ struct Step {
         const int P = a.pairs;
         int64_t channel;
         if (c < a.turned) {
-            const int j = SMALL ? (int)c * kPiece : min((int)c * kPiece, P - a.full);
+            const int j = SMALL ? (int)c * kPiece : (FEW ? 0 : min((int)c * kPiece, P - kPiece));
             at = t * P + j;
-            count = SMALL ? min(kPiece, P - j) : a.full;
+            count = SMALL ? min(kPiece, P - j) : (FEW ? P : kPiece);
             channel = HALF ? j : 2 * j;
         } else {
             const int j = a.copied + (int)(c - a.turned) * kPiece;
@@ -118,7 +121,7 @@ struct Step {
             v.to(g);
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) {
-                const bool real = SMALL ? e < count : e < a.full;
+                const bool real = SMALL ? e < count : (!FEW || e < a.pairs);
                 const float2 w = table[at + (real ? e : 0)];
                 float& p = HALF ? f[e] : (e < kPiece / 2 ? f[(2 * e) % kPiece] : g[(2 * e) % kPiece]);
                 float& q = HALF ? g[e] : (e < kPiece / 2 ? f[(2 * e + 1) % kPiece] : g[(2 * e + 1) % kPiece]);
@@ -133,9 +136,9 @@ struct Step {
             store_some(u, dst, first_run());
             store_some(v, dst + apart(a), second_run());
         } else {
-            if (count > 0 && HALF && a.full < kPiece) {
-                store_some(u, dst, a.full);
-                store_some(v, dst + apart(a), a.full);
+            if (FEW && HALF && count > 0) {
+                store_some(u, dst, a.pairs);
+                store_some(v, dst + apart(a), a.pairs);
             } else if (count == -kPiece || count > 0) {
                 u.store(dst);
                 if (count > 0) v.store(dst + apart(a));
@@ -148,13 +151,13 @@ struct Step {
     }
 };
 
-template <typename T, bool HALF, bool SMALL>
+template <typename T, bool HALF, int FORM>
 __global__ __launch_bounds__(kThreads) void k_rotary(RotaryDev a) {
     extern __shared__ float2 table[];  // [run][pairs]
     const uint32_t entry = blockIdx.x / a.tiles;
     const int64_t b = entry, first = (int64_t)(blockIdx.x - entry * a.tiles) * a.run;
     const int live = (int)min((int64_t)a.run, a.tokens - first);
-    Step<T, HALF, SMALL> s;
+    Step<T, HALF, FORM> s;
     auto fetch = [&](int k, uint32_t i, uint32_t all) {
         s.place(a, k, b, first, min(i, all - 1));  // past the end: the last step once more
         s.load(a);
@@ -187,13 +190,20 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryDev a) {
 
 inline uint32_t inverse_of(uint32_t d) { return d == 1 ? 0 : (uint32_t)(((1ULL << 32) + d - 1) / d); }
 
-template <typename T>
-void launch(const RotaryDev& a, bool half, bool small, unsigned blocks, hipStream_t s) {
+template <typename T, bool HALF>
+void launch(const RotaryDev& a, int form, unsigned blocks, hipStream_t s) {
     const size_t lds = (size_t)a.run * a.pairs * sizeof(float2);
-    if (half && small) k_rotary<T, true, true><<<blocks, kThreads, lds, s>>>(a);
-    else if (half) k_rotary<T, true, false><<<blocks, kThreads, lds, s>>>(a);
-    else if (small) k_rotary<T, false, true><<<blocks, kThreads, lds, s>>>(a);
-    else k_rotary<T, false, false><<<blocks, kThreads, lds, s>>>(a);
+    switch (form) {
+        case kWhole: k_rotary<T, HALF, kWhole><<<blocks, kThreads, lds, s>>>(a); break;
+        case kFew: k_rotary<T, HALF, kFew><<<blocks, kThreads, lds, s>>>(a); break;
+        default: k_rotary<T, HALF, kSmall><<<blocks, kThreads, lds, s>>>(a); break;
+    }
+}
+
+template <typename T>
+void launch(const RotaryDev& a, bool half, int form, unsigned blocks, hipStream_t s) {
+    if (half) launch<T, true>(a, form, blocks, s);
+    else launch<T, false>(a, form, blocks, s);
 }
 
 }  // namespace
@@ -222,9 +232,8 @@ extern "C" int p3d_rotary(const p3d_rotary_args* args, void* stream) {
     a.head_dim = g.head_dim;
     a.pairs = g.pairs;
     a.turned = (uint32_t)cdiv(g.pairs, kPiece);
-    const bool small = g.head_dim < 2 * kPiece;
-    a.full = g.pairs < kPiece ? g.pairs : kPiece;
-    a.copied = !small && !g.half && g.pairs < kPiece ? 2 * kPiece : 2 * g.pairs;
+    const int form = g.head_dim < 2 * kPiece ? kSmall : (g.pairs < kPiece ? kFew : kWhole);
+    a.copied = form == kFew && !g.half ? 2 * kPiece : 2 * g.pairs;
     a.chunks = a.turned + (uint32_t)cdiv(g.head_dim - a.copied, kPiece);
     a.chunks_inv = inverse_of(a.chunks);
     a.count = g.count;
@@ -260,9 +269,9 @@ extern "C" int p3d_rotary(const p3d_rotary_args* args, void* stream) {
     const unsigned blocks = (unsigned)g.batch * a.tiles;
     hipStream_t s = as_stream(stream);
     switch (g.dtype) {
-        case P3D_F32: launch<float>(a, g.half, small, blocks, s); break;
-        case P3D_F16: launch<_Float16>(a, g.half, small, blocks, s); break;
-        default: launch<__bf16>(a, g.half, small, blocks, s); break;
+        case P3D_F32: launch<float>(a, g.half, form, blocks, s); break;
+        case P3D_F16: launch<_Float16>(a, g.half, form, blocks, s); break;
+        default: launch<__bf16>(a, g.half, form, blocks, s); break;
     }
     return check_launch("p3d_rotary");
 }
