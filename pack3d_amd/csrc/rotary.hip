@@ -9,20 +9,17 @@
 // 2^-26 turns.
 //
 // A block takes a run of tokens: (cos, sin) of each of their pairs into LDS, once for
-// all heads of all tensors, then the heads, eight pairs (32 bytes of a 16-bit type) or
-// eight copied channels a thread and step, the first step's loads issued before the
-// angles are worked out.  A block takes the tokens of one step a thread: more blocks with
-// smaller tables measured faster than steps ahead within one (three bf16 tensors of
-// 262,144 x 4 x 48: 124 us; with two steps a thread 126, four 136, their loads together
-// 140), and the angles cost nothing next to the memory (138 and 139 us without and with
-// them).  Where eight does not divide the pairs, the last two steps of a head overlap and
-// store the same bits twice.  Bound by memory: 4 bytes an element in 16 bits, 4.9 TB/s.
+// all heads of all tensors, then the heads, 32 bytes a thread and step, the first step's
+// loads issued before the angles are worked out.  A block takes the tokens of one step a
+// thread: more blocks with smaller tables measured faster than steps ahead within one
+// (three bf16 tensors of 262,144 x 4 x 48: 124 us; with two steps a thread 126, four 136,
+// their loads together 140), and the angles cost nothing next to the memory (138 and 139
+// us without and with them).  Bound by memory: 4 bytes an element in 16 bits, 5.1 TB/s.
 #include "elements.hpp"
 
 namespace p3d {
 namespace {
 
-constexpr int kPiece = 8;
 constexpr int kThreads = 256;
 constexpr int kMaxTensors = 4;
 constexpr int kMaxTable = 4096;  // (cos, sin) of a block: 32 KiB
@@ -48,22 +45,26 @@ struct RotaryDev {
 // a / d for a < 2^32 / d, with inv = ceil(2^32 / d); d = 1 has inv = 0.
 __device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t inv) { return inv ? __umulhi(a, inv) : a; }
 
-// One step: eight pairs (two runs of eight channels, apart or adjacent), or eight channels
-// that are copied.  Heads with fewer than eight pairs have one step of them, which reads
-// runs of eight all the same: adjacent, it copies the channels behind the pairs too; apart,
-// it stores what is the pairs' (30M bf16 channels in heads of 16 with 3 pairs: 26 and 60
-// us; whole heads 27).  Copies of fewer than eight channels read the head's last eight and
-// store what is theirs.  Heads of fewer than 16 channels go an element at a time.
-enum Form { kWhole, kFew, kSmall };  // eight pairs or more; fewer; heads of fewer than 16 channels
+// One step: two runs of N channels, 16 bytes each: N pairs (apart by the pairs, or
+// adjacent), or 2N channels that are copied.  Where N does not divide the pairs, or 2N the
+// copied channels, the last two steps overlap and store the same bits twice.  Heads with
+// fewer than N pairs have one step of them, which reads whole runs all the same: adjacent,
+// it copies the channels behind the pairs too; apart, it stores what is the pairs' (30M
+// bf16 channels in heads of 16 with 3 pairs: 26 and 58 us; whole heads 27).  Fewer than 2N
+// copied channels: the step reads the head's last 2N and stores what is theirs.  Heads of
+// fewer than 2N channels go an element at a time.
+enum Form { kWhole, kFew, kSmall };  // N pairs or more; fewer; heads of fewer than 2N channels
 
 template <typename T, bool HALF, int FORM>
 struct Step {
+    static constexpr int N = Piece<T>::N;
     static constexpr bool FEW = FORM == kFew, SMALL = FORM == kSmall;
     const char* src;
     char* dst;
     uint32_t at;  // of the (cos, sin) of its first pair
     int count;    // pairs, or minus the channels to copy
-    Run<T, kPiece> u, v;
+    int gap;      // bytes from the first run to the second
+    Run<T, N> u, v;
 
     // k: the tensor, the same for the whole launch's step.
     __device__ __forceinline__ void place(const RotaryDev& a, int k, int64_t b, int64_t first, uint32_t i) {
@@ -71,60 +72,58 @@ struct Step {
         const uint32_t h = quotient(r, a.chunks_inv), c = r - h * a.chunks;
         const p3d_view &x = a.x[k], &y = a.y[k];
         const int P = a.pairs;
-        int64_t channel;
+        int channel;
         if (c < a.turned) {
-            const int j = SMALL ? (int)c * kPiece : (FEW ? 0 : min((int)c * kPiece, P - kPiece));
+            const int j = SMALL ? (int)c * N : (FEW ? 0 : min((int)c * N, P - N));
             at = t * P + j;
-            count = SMALL ? min(kPiece, P - j) : (FEW ? P : kPiece);
+            count = SMALL ? min(N, P - j) : (FEW ? P : N);
             channel = HALF ? j : 2 * j;
+            gap = (HALF ? P : N) * (int)sizeof(T);
         } else {
-            const int j = a.copied + (int)(c - a.turned) * kPiece;
+            const int j = a.copied + (int)(c - a.turned) * 2 * N, left = a.head_dim - a.copied;
             at = 0;
-            count = -min(kPiece, a.head_dim - j);
-            channel = SMALL ? j : min(j, a.head_dim - kPiece);
+            count = SMALL ? -min(2 * N, a.head_dim - j) : -min(2 * N, left);
+            channel = SMALL ? j : min(j, a.head_dim - 2 * N);
+            gap = N * (int)sizeof(T);
         }
         src = reinterpret_cast<const char*>(reinterpret_cast<const T*>(x.data) + b * x.sb + (int64_t)h * x.sh +
                                             (first + t) * x.sn + channel);
         dst = reinterpret_cast<char*>(reinterpret_cast<T*>(y.data) + b * y.sb + (int64_t)h * y.sh +
                                       (first + t) * y.sn + channel);
     }
-    // Bytes from the first run of eight channels to the second.
-    __device__ __forceinline__ int64_t apart(const RotaryDev& a) const {
-        return (HALF ? a.pairs : kPiece) * (int64_t)sizeof(T);
-    }
-    __device__ __forceinline__ static void load_some(Run<T, kPiece>& r, const char* p, int n) {
+    // Elements low to high - 1 of a run.
+    __device__ __forceinline__ static void load_some(Run<T, N>& r, const char* p, int high) {
 #pragma unroll
-        for (int e = 0; e < kPiece; ++e) r.v[e] = e < n ? reinterpret_cast<const T*>(p)[e] : from_f32<T>(0.f);
+        for (int e = 0; e < N; ++e) r.v[e] = e < high ? reinterpret_cast<const T*>(p)[e] : from_f32<T>(0.f);
     }
-    __device__ __forceinline__ static void store_some(const Run<T, kPiece>& r, char* p, int n) {
+    __device__ __forceinline__ static void store_some(const Run<T, N>& r, char* p, int low, int high) {
 #pragma unroll
-        for (int e = 0; e < kPiece; ++e)
-            if (e < n) reinterpret_cast<T*>(p)[e] = r.v[e];
+        for (int e = 0; e < N; ++e)
+            if (e >= low && e < high) reinterpret_cast<T*>(p)[e] = r.v[e];
     }
-    // Channels of the two runs, in the small form.
-    __device__ __forceinline__ int first_run() const { return count < 0 ? -count : (HALF ? count : min(2 * count, kPiece)); }
-    __device__ __forceinline__ int second_run() const { return count < 0 ? 0 : (HALF ? count : 2 * count - kPiece); }
+    // Channels of the two runs together where they are adjacent, of each where apart.
+    __device__ __forceinline__ int channels() const { return count < 0 ? -count : (HALF ? count : 2 * count); }
+    __device__ __forceinline__ int second() const { return HALF && count > 0 ? count : channels() - N; }
     __device__ __forceinline__ void load(const RotaryDev& a) {
         if constexpr (SMALL) {
-            load_some(u, src, first_run());
-            load_some(v, src + apart(a), second_run());
+            load_some(u, src, channels());
+            load_some(v, src + gap, second());
         } else {
             u.load(src);
-            // A step that copies reads its own run twice rather than none: no branch.
-            v.load(src + (count < 0 ? 0 : apart(a)));
+            v.load(src + gap);
         }
     }
     __device__ __forceinline__ void turn(const RotaryDev& a, const float2* table) {
         if (count > 0) {
-            float f[kPiece], g[kPiece];
+            float f[N], g[N];
             u.to(f);
             v.to(g);
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e) {
+            for (int e = 0; e < N; ++e) {
                 const bool real = SMALL ? e < count : (!FEW || e < a.pairs);
                 const float2 w = table[at + (real ? e : 0)];
-                float& p = HALF ? f[e] : (e < kPiece / 2 ? f[(2 * e) % kPiece] : g[(2 * e) % kPiece]);
-                float& q = HALF ? g[e] : (e < kPiece / 2 ? f[(2 * e + 1) % kPiece] : g[(2 * e + 1) % kPiece]);
+                float& p = HALF ? f[e] : (e < N / 2 ? f[(2 * e) % N] : g[(2 * e) % N]);
+                float& q = HALF ? g[e] : (e < N / 2 ? f[(2 * e + 1) % N] : g[(2 * e + 1) % N]);
                 const float s = p * w.x - q * w.y, t = p * w.y + q * w.x;
                 p = real ? s : p;
                 q = real ? t : q;
@@ -133,20 +132,17 @@ struct Step {
             v.from(g);
         }
         if constexpr (SMALL) {
-            store_some(u, dst, first_run());
-            store_some(v, dst + apart(a), second_run());
+            store_some(u, dst, 0, channels());
+            store_some(v, dst + gap, 0, second());
+        } else if (FEW && HALF && count > 0) {
+            store_some(u, dst, 0, a.pairs);
+            store_some(v, dst + gap, 0, a.pairs);
+        } else if (count > 0 || count == -2 * N) {
+            u.store(dst);
+            v.store(dst + gap);
         } else {
-            if (FEW && HALF && count > 0) {
-                store_some(u, dst, a.pairs);
-                store_some(v, dst + apart(a), a.pairs);
-            } else if (count == -kPiece || count > 0) {
-                u.store(dst);
-                if (count > 0) v.store(dst + apart(a));
-            } else {
-#pragma unroll
-                for (int e = 0; e < kPiece; ++e)
-                    if (e >= kPiece + count) reinterpret_cast<T*>(dst)[e] = u.v[e];
-            }
+            store_some(u, dst, 2 * N + count, N);
+            store_some(v, dst + gap, N + count, N);
         }
     }
 };
@@ -231,10 +227,11 @@ extern "C" int p3d_rotary(const p3d_rotary_args* args, void* stream) {
     a.tokens = g.tokens;
     a.head_dim = g.head_dim;
     a.pairs = g.pairs;
-    a.turned = (uint32_t)cdiv(g.pairs, kPiece);
-    const int form = g.head_dim < 2 * kPiece ? kSmall : (g.pairs < kPiece ? kFew : kWhole);
-    a.copied = form == kFew && !g.half ? 2 * kPiece : 2 * g.pairs;
-    a.chunks = a.turned + (uint32_t)cdiv(g.head_dim - a.copied, kPiece);
+    const int piece = 16 / dtype_size(g.dtype);
+    a.turned = (uint32_t)cdiv(g.pairs, piece);
+    const int form = g.head_dim < 2 * piece ? kSmall : (g.pairs < piece ? kFew : kWhole);
+    a.copied = form == kFew && !g.half ? 2 * piece : 2 * g.pairs;
+    a.chunks = a.turned + (uint32_t)cdiv(g.head_dim - a.copied, 2 * piece);
     a.chunks_inv = inverse_of(a.chunks);
     a.count = g.count;
     uint32_t most = 0;
