@@ -405,7 +405,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
                 const float mean1 = st[0], rstd1 = st[1], mean2 = st[2], rstd2 = st[3];
                 if constexpr (AHEAD) fetch(unit.first + min(i + GROUPS, last));
                 uint32_t bits = 0xffffffffu;
-                float b[E];  // keep b, and times the gate where it has one a token
+                float b[E];  // keep b
                 if constexpr (HAS_Y) {
                     if (has_post) {
 #pragma unroll

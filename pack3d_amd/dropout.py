@@ -49,7 +49,8 @@ def counter_dropout(x, p, seed):
     """x with each element dropped at rate p (a multiple of 2^-16, the nearest) and the
     others divided by 1 - p.  The same seed gives the same mask, in the backward too;
     another call needs another seed or offset.  fp32, fp16 and bf16, any shape (a
-    tensor that is not contiguous is copied first); differentiable (first order)."""
+    tensor that is not contiguous is copied first); differentiable (first order).
+    A rate that rounds to 0 gives x itself."""
     mask = mask_args(p, seed, x.device)
     if not mask[0] and x.is_cuda and x.dtype in _lib.DTYPES:
         return x

@@ -31,9 +31,15 @@ def assert_within(got, ref, bound, what):
 
 
 def keep_mask(count, threshold, seed, offset):
-    """Truth values of the elements that stay: Philox4x32-10 in unsigned 64-bit numpy arithmetic."""
+    """Truth values of the first elements that stay."""
+    return keep_mask_at(0, count, threshold, seed, offset)
+
+
+def keep_mask_at(first, count, threshold, seed, offset):
+    """Truth values of the elements from `first` (a multiple of 8) on that stay: Philox4x32-10 in unsigned 64-bit
+    numpy arithmetic."""
     low, shift = np.uint64(0xFFFFFFFF), np.uint64(32)
-    group = np.arange(-(-count // 8), dtype=np.uint64)
+    group = first // 8 + np.arange(-(-count // 8), dtype=np.uint64)
     c = [group & low, group >> shift, np.full_like(group, offset & 0xFFFFFFFF), np.full_like(group, offset >> 32)]
     k = [seed & 0xFFFFFFFF, seed >> 32]
     for _ in range(10):

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 import pack3d_amd as p3d
-from tests._block_reference import (assert_within, block_reference, half_step, keep_mask, smallest, sum_bound)
+from tests._block_reference import (assert_within, block_reference, half_step, keep_mask, keep_mask_at, smallest,
+                                    sum_bound)
 
 pytestmark = pytest.mark.gpu
 
@@ -405,3 +406,40 @@ def test_calls_from_two_threads(gpu):
     for a, b in zip(alone, got):
         for p, q in zip(a, b):
             assert torch.equal(p, q)
+
+
+def test_rows_beyond_four_gigabytes(gpu):
+    """Rows 8 MiB apart (their last bytes past 2^33) read as contiguous copies of them do."""
+    rows, stride = 1100, 1 << 22
+    big = torch.empty(rows * stride, dtype=BF16, device=gpu)
+    x, y, gate, up = (big.as_strided((rows, 72), (stride, 1), 512 * i) for i in range(4))
+    gen = torch.Generator(device=gpu).manual_seed(1)
+    for t in (x, y, gate, up):
+        t.copy_(torch.randn(rows, 72, generator=gen, device=gpu))
+
+    def run(x, y, gate, up):
+        x, y, gate = (t.detach().requires_grad_() for t in (x, y, gate))
+        out, n = p3d.block_residual(x, y, post_norm=p3d.Norm("layer"), gate=gate, p=0.1, seed=5, next_norm=p3d.Norm("rms"))
+        return (out, n, *torch.autograd.grad((out, n), (x, y, gate), (up, up)))
+    for a, b in zip(run(x, y, gate, up), run(*(t.contiguous() for t in (x, y, gate, up)))):
+        assert torch.equal(a, b)
+    far = big.as_strided((5, 64), (1 << 29, 1))  # a stride that is copied before the kernel
+    far.copy_(torch.randn(5, 64, device=gpu))
+    assert torch.equal(p3d.block_norm(far, p3d.Norm("rms")), p3d.block_norm(far.contiguous(), p3d.Norm("rms")))
+
+
+def test_outputs_beyond_four_gigabytes(gpu):
+    """2^31 and some elements: the last rows of each output as a call on those rows alone gives them."""
+    rows, dim = 33_600_000, 64
+    x = torch.empty(rows, dim, dtype=BF16, device=gpu)
+    x.normal_()
+    n = p3d.block_norm(x, p3d.Norm("layer"))
+    assert torch.equal(n[-100:], p3d.block_norm(x[-100:], p3d.Norm("layer")))
+    del n
+    y = p3d.counter_dropout(x, 0.25, (3, 4))
+    first = (rows - 2) * dim
+    keep = keep_mask_at(first, 2 * dim, 16384, 3, 4)
+    inv = torch.tensor(65536.0 / 49152.0, dtype=F32)
+    assert torch.equal(y[-2:].cpu().flatten(), torch.where(keep, x[-2:].cpu().flatten().float() * inv, 0.0).to(BF16))
+    out = p3d.block_residual(torch.zeros_like(x), x, p=0.25, seed=(3, 4))
+    assert torch.equal(out[-2:], y[-2:])

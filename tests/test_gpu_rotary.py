@@ -116,6 +116,16 @@ def test_strides(gpu):
     assert p3d.apply_rotary(x[:0], positions[:1], freqs).shape == (0, 4, n, d)
 
 
+def test_rows_beyond_four_gigabytes(gpu):
+    """Tokens 8 MiB apart read as a contiguous copy of them does."""
+    n, stride = 1100, 1 << 22
+    x = torch.empty(n * stride, dtype=torch.bfloat16, device=gpu).as_strided((1, 2, n, 64), (0, 64, stride, 1))
+    x.copy_(torch.randn(1, 2, n, 64, device=gpu))
+    positions, freqs = torch.arange(n, device=gpu), p3d.rotary_frequencies(20)[0].to(gpu)
+    assert torch.equal(p3d.apply_rotary(x, positions, freqs, layout="half"),
+                       p3d.apply_rotary(x.contiguous(), positions, freqs, layout="half"))
+
+
 def test_some_gradients_only(gpu):
     q, k = (torch.randn(1, 2, 9, 16, device=gpu) for _ in range(2))
     k.requires_grad_()
