@@ -635,6 +635,11 @@ typedef struct p3d_block_args {
     float* work;
 } p3d_block_args;
 
+/* Workgroups that the current device runs at a time of the kernel that p3d_block_fwd, or
+ * with backward p3d_block_bwd, launches for these arguments (splits and grid: any that
+ * are in range): a good `grid` for the backward.  Launches nothing. */
+int p3d_block_resident(const p3d_block_args* args, int32_t backward, int32_t* count);
+
 int p3d_block_fwd(const p3d_block_args* args, void* stream);
 int p3d_block_bwd(const p3d_block_args* args, void* stream);
 

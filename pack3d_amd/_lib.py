@@ -168,6 +168,7 @@ SIGNATURES = {
     "p3d_gate_bwd": ([_P, c_int32, View, c_int32, _P, _P, c_int32, c_int32, c_int64, _P], c_int32),
     "p3d_cast": ([ctypes.POINTER(CastJob), c_int32, _P], c_int32),
     "p3d_dropout_apply": ([_P, _P, c_int64, c_int32, ctypes.POINTER(Dropout), _P], c_int32),
+    "p3d_block_resident": ([ctypes.POINTER(BlockArgs), c_int32, ctypes.POINTER(c_int32)], c_int32),
     "p3d_block_fwd": ([ctypes.POINTER(BlockArgs), _P], c_int32),
     "p3d_block_bwd": ([ctypes.POINTER(BlockArgs), _P], c_int32),
     "p3d_rotary": ([ctypes.POINTER(RotaryArgs), _P], c_int32),
@@ -313,8 +314,8 @@ def ops():
         if _torch_ops.abi_version() != ABI_VERSION:
             raise RuntimeError("pack3d_amd torch binding ABI mismatch; rebuild it")
         _torch_ops.bind_library(*(ctypes.cast(getattr(handle, name), c_void_p).value for name in
-                                  ("p3d_block_fwd", "p3d_block_bwd", "p3d_dropout_apply", "p3d_rotary",
-                                   "p3d_last_error")))
+                                  ("p3d_block_fwd", "p3d_block_bwd", "p3d_block_resident", "p3d_dropout_apply",
+                                   "p3d_rotary", "p3d_last_error")))
         _ops = _torch_ops
     return _ops
 

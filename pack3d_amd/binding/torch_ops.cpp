@@ -20,7 +20,9 @@
 
 #include <array>
 #include <cmath>
+#include <mutex>
 #include <optional>
+#include <unordered_map>
 
 #include "../../include/pack3d_hip.h"
 
@@ -36,14 +38,17 @@ typedef std::optional<Tensor> MaybeTensor;
 struct Library {
     decltype(&p3d_block_fwd) block_fwd = nullptr;
     decltype(&p3d_block_bwd) block_bwd = nullptr;
+    decltype(&p3d_block_resident) block_resident = nullptr;
     decltype(&p3d_dropout_apply) dropout_apply = nullptr;
     decltype(&p3d_rotary) rotary = nullptr;
     decltype(&p3d_last_error) last_error = nullptr;
 } lib;
 
-void bind_library(int64_t block_fwd, int64_t block_bwd, int64_t dropout_apply, int64_t rotary, int64_t last_error) {
+void bind_library(int64_t block_fwd, int64_t block_bwd, int64_t block_resident, int64_t dropout_apply, int64_t rotary,
+                  int64_t last_error) {
     lib.block_fwd = reinterpret_cast<decltype(lib.block_fwd)>(block_fwd);
     lib.block_bwd = reinterpret_cast<decltype(lib.block_bwd)>(block_bwd);
+    lib.block_resident = reinterpret_cast<decltype(lib.block_resident)>(block_resident);
     lib.dropout_apply = reinterpret_cast<decltype(lib.dropout_apply)>(dropout_apply);
     lib.rotary = reinterpret_cast<decltype(lib.rotary)>(rotary);
     lib.last_error = reinterpret_cast<decltype(lib.last_error)>(last_error);
@@ -107,20 +112,22 @@ Tensor or_undefined(const MaybeTensor& t) { return t.has_value() ? *t : Tensor()
 constexpr int64_t kMaxDim = 8192;
 constexpr int64_t kMaxStride = 1LL << 29;  // elements between rows
 
-// Ranges that a sample's rows are cut into, and workgroups.
-std::pair<int64_t, int64_t> block_split(int64_t samples, int64_t tokens, int64_t dim, bool backward) {
-    int64_t threads = dim < 4 ? 4 : 2;  // of a row
+int64_t row_threads(int64_t dim) {
+    int64_t threads = dim < 4 ? 4 : 2;
     while (threads < 1024 && dim > threads * 8) threads *= 2;
+    return threads;
+}
+
+// Ranges that a sample's rows are cut into, and workgroups.  round: the workgroups that
+// the backward is to have; 0 for the forward.
+std::pair<int64_t, int64_t> block_split(int64_t samples, int64_t tokens, int64_t dim, int64_t round) {
+    const int64_t threads = row_threads(dim);
     const int64_t rows = threads <= 64 ? 256 / threads : 1;  // that a workgroup holds at a time
     const int64_t per_sample = (tokens + rows - 1) / rows, steps = per_sample * samples;
-    int64_t wanted;
-    if (backward) {
-        // One round of what the GPU runs at a time (two waves a SIMD): each workgroup
-        // leaves a row of partial parameter gradients.
-        wanted = std::max<int64_t>(256, (1 << 17) / (threads > 64 ? threads : 256));
-    } else if (threads > 64) {
+    int64_t wanted = round;
+    if (!round && threads > 64) {
         wanted = std::max<int64_t>(512, (1 << 18) / threads);
-    } else {
+    } else if (!round) {
         // Several rounds, of at least four steps each once every CU has work: a workgroup
         // begins by loading the parameters (4,913 x 3 rows of 327: 21 us in 921, 25 in 3,685).
         wanted = std::max(std::min<int64_t>(1024, steps), std::min<int64_t>(4096, steps / 4));
@@ -208,6 +215,33 @@ p3d_block_args bind_block(const BlockSpec& spec, const Inputs& in, variable_list
     return a;
 }
 
+// Workgroups of the backward: one round, since each leaves a row of partial parameter
+// gradients and a second round waits on a few.  A lone norm takes two waves a SIMD
+// (32,000 rows of 1,000, forward and backward: 109 us; 111 with three, 128 with the four
+// that run at a time).  An end takes what the GPU runs of its kernel at a time, three at
+// most, asked once for each kind of call (gated, without a next norm, rows of 192 and
+// 1,024: 114 and 106 us with three, 132 and 118 with two).
+int64_t backward_round(const Tensor& x, const p3d_block_args& args) {
+    static std::mutex mutex;
+    static std::unordered_map<uint64_t, int32_t> known;
+    const int64_t threads = row_threads(args.dim);
+    const int64_t simd_waves = 64 * 1024 / (threads > 64 ? threads : 256);  // workgroups that are a wave on each
+    if (!args.y) return std::max<int64_t>(256, 2 * simd_waves);
+    const int gated = args.gate_kind == P3D_GATE_TOKEN || args.gate_kind == P3D_GATE_FULL;
+    const uint64_t key = (((((uint64_t)x.device().index() << 16 | (uint64_t)args.dim) << 2 | (uint64_t)args.outer) << 2 |
+                           (uint64_t)args.inner) << 1 | gated) << 1 | (args.dn ? 1 : 0);
+    std::lock_guard<std::mutex> lock(mutex);
+    int32_t& count = known[key];
+    if (!count) {
+        const c10::OptionalDeviceGuard guard(x.device());
+        p3d_block_args a = args;
+        a.splits = a.grid = 1;
+        const int rc = lib.block_resident(&a, 1, &count);
+        TORCH_CHECK(rc == 0, "p3d_block_resident failed (", rc, "): ", lib.last_error());
+    }
+    return std::min(std::max<int64_t>(256, 3 * simd_waves), (int64_t)count);
+}
+
 struct BlockOutputs {
     Tensor out, n, stats;
 };
@@ -226,7 +260,7 @@ BlockOutputs block_forward(const BlockSpec& spec, const Inputs& in, bool save) {
         a.out = o.out.defined() ? o.out.data_ptr() : nullptr;
         a.n = o.n.defined() ? o.n.data_ptr() : nullptr;
         a.stats = save ? static_cast<float*>(o.stats.data_ptr()) : nullptr;
-        const auto [splits, grid] = block_split(a.samples, a.tokens, a.dim, false);
+        const auto [splits, grid] = block_split(a.samples, a.tokens, a.dim, 0);
         a.splits = (int32_t)splits;
         a.grid = (int32_t)grid;
         launch("p3d_block_fwd", x, lib.block_fwd, &a);
@@ -301,11 +335,6 @@ struct BlockBackward : public Node {
             result[kParams[i]] = g;
         }
         if (rows) {
-            const auto [splits, grid] = block_split(a.samples, a.tokens, dim, true);
-            a.splits = (int32_t)splits;
-            a.grid = (int32_t)grid;
-            const int64_t sums = grid * 5 + (spec.gate_kind == P3D_GATE_SAMPLE ? splits * a.samples : 0);
-            const Tensor work = at::empty({sums * dim}, x.options().dtype(at::kFloat).requires_grad(false));
             if (y.defined()) {
                 // Only n was used: a row of zeros, for every row.
                 if (!dout.defined()) dout = at::zeros({1, dim}, x.options().requires_grad(false)).expand({rows, dim});
@@ -316,6 +345,11 @@ struct BlockBackward : public Node {
                 dn = dn.to(spec.inner);
                 std::tie(a.dn, a.dn_stride) = rows_of(dn, dim, keep);
             }
+            const auto [splits, grid] = block_split(a.samples, a.tokens, dim, backward_round(x, a));
+            a.splits = (int32_t)splits;
+            a.grid = (int32_t)grid;
+            const int64_t sums = grid * 5 + (spec.gate_kind == P3D_GATE_SAMPLE ? splits * a.samples : 0);
+            const Tensor work = at::empty({sums * dim}, x.options().dtype(at::kFloat).requires_grad(false));
             a.stats = static_cast<float*>(stats.data_ptr());
             a.work = static_cast<float*>(work.data_ptr());
             launch("p3d_block_bwd", x, lib.block_bwd, &a);

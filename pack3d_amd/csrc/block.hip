@@ -3,11 +3,11 @@
 
 namespace p3d {
 
-extern template int launch_block<float, float>(const BlockDev&, bool, unsigned, hipStream_t);
-extern template int launch_block<_Float16, _Float16>(const BlockDev&, bool, unsigned, hipStream_t);
-extern template int launch_block<__bf16, __bf16>(const BlockDev&, bool, unsigned, hipStream_t);
-extern template int launch_block<float, _Float16>(const BlockDev&, bool, unsigned, hipStream_t);
-extern template int launch_block<float, __bf16>(const BlockDev&, bool, unsigned, hipStream_t);
+extern template int launch_block<float, float>(const BlockDev&, const BlockLaunch&);
+extern template int launch_block<_Float16, _Float16>(const BlockDev&, const BlockLaunch&);
+extern template int launch_block<__bf16, __bf16>(const BlockDev&, const BlockLaunch&);
+extern template int launch_block<float, _Float16>(const BlockDev&, const BlockLaunch&);
+extern template int launch_block<float, __bf16>(const BlockDev&, const BlockLaunch&);
 
 namespace {
 
@@ -74,26 +74,42 @@ int block_dev(const p3d_block_args* args, BlockDev& a) {
     return P3D_OK;
 }
 
-int launch(const p3d_block_args& g, const BlockDev& a, bool backward, void* stream) {
-    hipStream_t s = as_stream(stream);
-    const unsigned grid = (unsigned)g.grid;
-    if (g.outer == P3D_F16) return launch_block<_Float16, _Float16>(a, backward, grid, s);
-    if (g.outer == P3D_BF16) return launch_block<__bf16, __bf16>(a, backward, grid, s);
-    if (g.inner == P3D_F16) return launch_block<float, _Float16>(a, backward, grid, s);
-    if (g.inner == P3D_BF16) return launch_block<float, __bf16>(a, backward, grid, s);
-    return launch_block<float, float>(a, backward, grid, s);
+int launch(const p3d_block_args& g, const BlockDev& a, const BlockLaunch& l) {
+    if (g.outer == P3D_F16) return launch_block<_Float16, _Float16>(a, l);
+    if (g.outer == P3D_BF16) return launch_block<__bf16, __bf16>(a, l);
+    if (g.inner == P3D_F16) return launch_block<float, _Float16>(a, l);
+    if (g.inner == P3D_BF16) return launch_block<float, __bf16>(a, l);
+    return launch_block<float, float>(a, l);
 }
 
 }  // namespace
+
+int resident_workgroups(const void* kernel, int threads, int32_t* count) {
+    int dev = 0, cus = 0, per_cu = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
+    if (e == hipSuccess) e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, 0);
+    if (e != hipSuccess) return fail(P3D_EHIP, std::string("p3d_block_resident: ") + hipGetErrorString(e));
+    *count = (cus > 0 ? cus : 1) * (per_cu > 0 ? per_cu : 1);
+    return P3D_OK;
+}
+
 }  // namespace p3d
 
 using namespace p3d;
+
+extern "C" int p3d_block_resident(const p3d_block_args* args, int32_t backward, int32_t* count) {
+    BlockDev a;
+    if (const int rc = block_dev(args, a)) return rc;
+    P3D_REQUIRE(count, "null pointer argument");
+    return launch(*args, a, BlockLaunch{backward != 0, 0, nullptr, count});
+}
 
 extern "C" int p3d_block_fwd(const p3d_block_args* args, void* stream) {
     BlockDev a;
     if (const int rc = block_dev(args, a)) return rc;
     P3D_REQUIRE((!a.y || a.out) && (!a.next.kind || a.n), "null output");
-    return launch(*args, a, false, stream);
+    return launch(*args, a, BlockLaunch{false, (unsigned)args->grid, as_stream(stream), nullptr});
 }
 
 extern "C" int p3d_block_bwd(const p3d_block_args* args, void* stream) {
@@ -126,6 +142,6 @@ extern "C" int p3d_block_bwd(const p3d_block_args* args, void* stream) {
         jobs[count++] = p3d_sum_job{a.dgate_part, a.dgate, a.splits, cols, (int32_t)cols, a.gate_dtype};
     }
     P3D_REQUIRE(!count || g.work, "work is missing");
-    if (const int rc = launch(g, a, true, stream)) return rc;
+    if (const int rc = launch(g, a, BlockLaunch{true, (unsigned)g.grid, as_stream(stream), nullptr})) return rc;
     return count ? p3d_sum_rows(jobs, count, stream) : P3D_OK;
 }

@@ -38,8 +38,18 @@ struct BlockDev {
     float* part;        // [grid][5][dim]: post weight, post bias, scale, next weight, next bias
 };
 
+struct BlockLaunch {
+    bool backward;
+    unsigned grid;
+    hipStream_t stream;
+    int32_t* resident;  // not NULL: no launch, the workgroups of the kernel that run at a time
+};
+
+// Workgroups of a kernel that the current device runs at a time.
+int resident_workgroups(const void* kernel, int threads, int32_t* count);
+
 // Launches the kernels of one pair of types (block_<outer>_<inner>.hip).
 template <typename TX, typename TY>
-int launch_block(const BlockDev& a, bool backward, unsigned grid, hipStream_t s);
+int launch_block(const BlockDev& a, const BlockLaunch& l);
 
 }  // namespace p3d

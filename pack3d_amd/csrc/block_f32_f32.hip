@@ -1,5 +1,5 @@
 #include "block_kernels.hpp"
 
 namespace p3d {
-template int launch_block<float, float>(const BlockDev&, bool, unsigned, hipStream_t);
+template int launch_block<float, float>(const BlockDev&, const BlockLaunch&);
 }

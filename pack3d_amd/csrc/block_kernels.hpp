@@ -545,24 +545,29 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
     if (NEXT && a.next.bias) gather(db2, part + 4 * (int64_t)a.dim);
 }
 
+// Launches a kernel, or counts the workgroups of it that the GPU runs at a time.
+template <typename K>
+int launch_kernel(K kernel, int threads, const BlockDev& a, const BlockLaunch& l, const char* what) {
+    if (l.resident) return resident_workgroups(reinterpret_cast<const void*>(kernel), threads, l.resident);
+    kernel<<<l.grid, threads, 0, l.stream>>>(a);
+    return check_launch(what);
+}
+
 template <typename TX, typename TY, int TPR, int E, int FORM>
-int launch_form(const BlockDev& a, bool backward, unsigned grid, hipStream_t s) {
+int launch_form(const BlockDev& a, const BlockLaunch& l) {
     constexpr int threads = block_threads(TPR);
-    if (backward) {
-        if (FORM == kNorm || a.dn) k_block_bwd<TX, TY, TPR, E, FORM, true><<<grid, threads, 0, s>>>(a);
-        else k_block_bwd<TX, TY, TPR, E, FORM, FORM == kNorm><<<grid, threads, 0, s>>>(a);
-        return check_launch("p3d_block_bwd");
-    }
-    k_block_fwd<TX, TY, TPR, E, FORM><<<grid, threads, 0, s>>>(a);
-    return check_launch("p3d_block_fwd");
+    if (!l.backward) return launch_kernel(k_block_fwd<TX, TY, TPR, E, FORM>, threads, a, l, "p3d_block_fwd");
+    if (FORM == kNorm || a.dn)
+        return launch_kernel(k_block_bwd<TX, TY, TPR, E, FORM, true>, threads, a, l, "p3d_block_bwd");
+    return launch_kernel(k_block_bwd<TX, TY, TPR, E, FORM, FORM == kNorm>, threads, a, l, "p3d_block_bwd");
 }
 
 template <typename TX, typename TY, int TPR, int E>
-int launch_as(const BlockDev& a, bool backward, unsigned grid, hipStream_t s) {
-    if (!a.y) return launch_form<TX, TY, TPR, E, kNorm>(a, backward, grid, s);
+int launch_as(const BlockDev& a, const BlockLaunch& l) {
+    if (!a.y) return launch_form<TX, TY, TPR, E, kNorm>(a, l);
     if (a.gate_kind == P3D_GATE_TOKEN || a.gate_kind == P3D_GATE_FULL)
-        return launch_form<TX, TY, TPR, E, kEndGated>(a, backward, grid, s);
-    return launch_form<TX, TY, TPR, E, kEnd>(a, backward, grid, s);
+        return launch_form<TX, TY, TPR, E, kEndGated>(a, l);
+    return launch_form<TX, TY, TPR, E, kEnd>(a, l);
 }
 
 }  // namespace
@@ -574,27 +579,27 @@ int launch_as(const BlockDev& a, bool backward, unsigned grid, hipStream_t s) {
 // 25,000 rows of 1,280 took 215 us in three waves, 170 in four of which two have no
 // channels.  block_split in binding/torch_ops.cpp deals out rows by the same widths.
 template <typename TX, typename TY>
-int launch_block(const BlockDev& a, bool backward, unsigned grid, hipStream_t s) {
+int launch_block(const BlockDev& a, const BlockLaunch& l) {
     const int d = a.dim;
-    if (d < 4) return launch_as<TX, TY, 4, 1>(a, backward, grid, s);
-    if (d < 8) return launch_as<TX, TY, 2, 4>(a, backward, grid, s);
-    if (d <= 16) return launch_as<TX, TY, 2, 8>(a, backward, grid, s);
-    if (d <= 32) return launch_as<TX, TY, 4, 8>(a, backward, grid, s);
-    if (d <= 64) return launch_as<TX, TY, 8, 8>(a, backward, grid, s);
-    if (d <= 96) return launch_as<TX, TY, 16, 6>(a, backward, grid, s);
-    if (d <= 128) return launch_as<TX, TY, 16, 8>(a, backward, grid, s);
-    if (d <= 192) return launch_as<TX, TY, 32, 6>(a, backward, grid, s);
-    if (d <= 256) return launch_as<TX, TY, 32, 8>(a, backward, grid, s);
-    if (d <= 384) return launch_as<TX, TY, 64, 6>(a, backward, grid, s);
-    if (d <= 512) return launch_as<TX, TY, 64, 8>(a, backward, grid, s);
-    if (d <= 128 * 6) return launch_as<TX, TY, 128, 6>(a, backward, grid, s);
-    if (d <= 128 * 8) return launch_as<TX, TY, 128, 8>(a, backward, grid, s);
-    if (d <= 256 * 6) return launch_as<TX, TY, 256, 6>(a, backward, grid, s);
-    if (d <= 256 * 8) return launch_as<TX, TY, 256, 8>(a, backward, grid, s);
-    if (d <= 512 * 6) return launch_as<TX, TY, 512, 6>(a, backward, grid, s);
-    if (d <= 512 * 8) return launch_as<TX, TY, 512, 8>(a, backward, grid, s);
-    if (d <= 1024 * 6) return launch_as<TX, TY, 1024, 6>(a, backward, grid, s);
-    return launch_as<TX, TY, 1024, 8>(a, backward, grid, s);
+    if (d < 4) return launch_as<TX, TY, 4, 1>(a, l);
+    if (d < 8) return launch_as<TX, TY, 2, 4>(a, l);
+    if (d <= 16) return launch_as<TX, TY, 2, 8>(a, l);
+    if (d <= 32) return launch_as<TX, TY, 4, 8>(a, l);
+    if (d <= 64) return launch_as<TX, TY, 8, 8>(a, l);
+    if (d <= 96) return launch_as<TX, TY, 16, 6>(a, l);
+    if (d <= 128) return launch_as<TX, TY, 16, 8>(a, l);
+    if (d <= 192) return launch_as<TX, TY, 32, 6>(a, l);
+    if (d <= 256) return launch_as<TX, TY, 32, 8>(a, l);
+    if (d <= 384) return launch_as<TX, TY, 64, 6>(a, l);
+    if (d <= 512) return launch_as<TX, TY, 64, 8>(a, l);
+    if (d <= 128 * 6) return launch_as<TX, TY, 128, 6>(a, l);
+    if (d <= 128 * 8) return launch_as<TX, TY, 128, 8>(a, l);
+    if (d <= 256 * 6) return launch_as<TX, TY, 256, 6>(a, l);
+    if (d <= 256 * 8) return launch_as<TX, TY, 256, 8>(a, l);
+    if (d <= 512 * 6) return launch_as<TX, TY, 512, 6>(a, l);
+    if (d <= 512 * 8) return launch_as<TX, TY, 512, 8>(a, l);
+    if (d <= 1024 * 6) return launch_as<TX, TY, 1024, 6>(a, l);
+    return launch_as<TX, TY, 1024, 8>(a, l);
 }
 
 }  // namespace p3d

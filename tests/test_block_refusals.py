@@ -144,8 +144,8 @@ def test_encoding_refusals(kw):
 
 
 @pytest.mark.parametrize("samples,tokens", [(1, 1), (1, 7), (3, 4913), (5000, 1), (1, 2 ** 31 - 1), (100000, 3)])
-@pytest.mark.parametrize("dim", [1, 64, 192, 512, 513, 8192])
-@pytest.mark.parametrize("backward", [False, True])
-def test_splits_stay_within_what_the_kernels_take(samples, tokens, dim, backward):
-    splits, grid = _lib.ops().block_split(samples, tokens, dim, backward)
+@pytest.mark.parametrize("dim", [1, 5, 64, 192, 512, 513, 8192])
+@pytest.mark.parametrize("round_", [0, 1, 256, 768, 2048])
+def test_splits_stay_within_what_the_kernels_take(samples, tokens, dim, round_):
+    splits, grid = _lib.ops().block_split(samples, tokens, dim, round_)
     assert 1 <= splits <= tokens and 1 <= grid <= splits * samples and splits * samples < 2 ** 31
