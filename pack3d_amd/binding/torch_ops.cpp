@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <array>
@@ -100,6 +101,20 @@ variable_list first_order(variable_list&& grads, bool create_graph, const variab
             torch::autograd::set_history(g, error);
         }
     return std::move(grads);
+}
+
+// A backward that is captured must not hand a gradient to a node of the default stream: a
+// leaf keeps the stream of its first use for as long as a graph of that use is alive, and
+// autograd would make the default stream wait on the capture, which ends the process.
+void refuse_default_stream(const Node& node) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (size_t i = 0; i < node.num_outputs(); ++i) {
+        if (!node.task_should_compute_output(i)) continue;
+        const auto stream = node.next_edge(i).function->stream();
+        TORCH_CHECK(!stream || *stream != c10::Stream(c10::Stream::DEFAULT, stream->device()),
+                    "a backward pass is captured into a graph while an eager graph of the same tensors, made on the "
+                    "default stream, is alive: drop its outputs first, or make it on another stream");
+    }
 }
 
 void no_forward_mode(const MaybeTensor& t) {
@@ -287,6 +302,7 @@ struct BlockBackward : public Node {
 
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
+        refuse_default_stream(*this);
         const bool create_graph = c10::GradMode::is_enabled();
         const c10::AutoGradMode off(false);
         auto self = shared_from_this();
@@ -479,6 +495,7 @@ struct DropoutBackward : public Node {
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
+        refuse_default_stream(*this);
         const Tensor seed = state.unpack(shared_from_this());
         if (!grads[0].defined()) return {Tensor()};
         if (seed.defined()) mask.state = static_cast<const int64_t*>(seed.const_data_ptr());
@@ -546,6 +563,7 @@ struct RotaryBackward : public Node {
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
+        refuse_default_stream(*this);
         const bool create_graph = c10::GradMode::is_enabled();
         const Tensor p = positions.unpack(shared_from_this()), f = freqs.unpack(shared_from_this());
         args.positions = p.const_data_ptr();

@@ -321,6 +321,35 @@ def test_training_step_in_a_graph(gpu):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("way", ["norm", "residual", "dropout", "rotary"])
+def test_captured_backward_while_an_eager_graph_lives(gpu, way):
+    """Refused while an eager graph of the leaf on the default stream is alive, and right once it is dropped."""
+    freqs, positions = p3d.rotary_frequencies(8)[0].to(gpu), torch.arange(6, device=gpu)
+    call = {"norm": lambda x: p3d.block_norm(x, p3d.Norm("rms")),
+            "residual": lambda x: p3d.block_residual(x, x.detach() * 2, p=0.3, seed=4, alpha=2.0),
+            "dropout": lambda x: p3d.counter_dropout(x, 0.3, 4),
+            "rotary": lambda x: p3d.apply_rotary(x, positions, freqs)}[way]
+    x = torch.randn(1, 2, 6, 16, device=gpu) if way == "rotary" else torch.randn(2, 6, 16, device=gpu)
+    x.requires_grad_()
+    up = torch.randn_like(x)
+    want, = torch.autograd.grad(call(x), x, up)
+    alive = call(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured into a graph while an eager graph"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(call(x), x, up)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(call(x), x, up)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_inputs_changed_before_the_backward_raise(gpu):
     x, y = (torch.randn(1, 4, 16, device=gpu, requires_grad=True) for _ in range(2))
     seed = torch.tensor([1, 2], device=gpu)
