@@ -14,7 +14,11 @@
 // reading it, and not rounded); the statistics come from the forward.
 //
 // Both are bound by memory: x and y (and dout and dn) are read, out and n (dx and dy)
-// written once.
+// written once.  262,144 rows of 192, fp32 x over bf16 y, with a post norm, dropout, a
+// gate per sample, scale and the next norm: forward 604 MB in 122 us, backward 906 MB in
+// 194 (4.9 and 4.7 TB/s; a large copy reaches 5.4), and 8 us for the partial sums.
+// 8,192 rows of 4,096 in bf16 with a gate per token and two RMSNorms: 56 and 91 us for
+// 268 and 403 MB (4.8 and 4.4).
 //
 // TPR threads share a row and hold E consecutive channels each, so a row is read
 // once into registers whatever its width.  Rows of up to 512 channels lie within a

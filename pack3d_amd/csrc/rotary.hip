@@ -12,9 +12,10 @@
 // all heads of all tensors, then the heads, 32 bytes a thread and step, the first step's
 // loads issued before the angles are worked out.  A block takes the tokens of one step a
 // thread: more blocks with smaller tables measured faster than steps ahead within one
-// (three bf16 tensors of 262,144 x 4 x 48: 124 us; with two steps a thread 126, four 136,
+// (three bf16 tensors of 262,144 x 4 x 48: one step 124 us, two a thread 126, four 136,
 // their loads together 140), and the angles cost nothing next to the memory (138 and 139
-// us without and with them).  Bound by memory: 4 bytes an element in 16 bits, 5.1 TB/s.
+// us without and with them; these figures before 16-byte runs, the same tensors now take
+// 120 us).  Bound by memory: 4 bytes an element in 16 bits, 5.1 TB/s.
 #include "elements.hpp"
 
 namespace p3d {

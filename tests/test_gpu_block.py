@@ -321,6 +321,26 @@ def test_training_step_in_a_graph(gpu):
         torch.cuda.synchronize()
 
 
+def test_first_step_of_its_kind_in_a_graph(gpu):
+    """A width and gate that nothing ran before, captured at once."""
+    x, y, gate, up = (torch.randn(300, 1001, device=gpu).half() for _ in range(4))
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, y, gate)]
+        out = p3d.block_residual(leaves[0], leaves[1], gate=leaves[2], p=0.25, seed=5, alpha=0.5)
+        return (out.detach(), *torch.autograd.grad(out, leaves, up))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    want = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+            a.zero_()
+
+
 @pytest.mark.parametrize("way", ["norm", "residual", "dropout", "rotary"])
 def test_captured_backward_while_an_eager_graph_lives(gpu, way):
     """Refused while an eager graph of the leaf on the default stream is alive, and right once it is dropped."""
