@@ -314,10 +314,30 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
     const char* pdn = reinterpret_cast<const char*>(a.dn) + c * sizeof(TY);
     char* pdx = reinterpret_cast<char*>(a.dx) + c * sizeof(TX);
     char* pdy = reinterpret_cast<char*>(a.dy) + c * sizeof(TY);
-    float par[3][E];
-    load_params<E, 3>({a.next.weight, HAS_Y ? a.post.weight : nullptr, HAS_Y ? a.post.bias : nullptr}, a.param, c,
-                      {1.f, 1.f, 0.f}, par);
-    const float(&w2)[E] = par[0], (&w1)[E] = par[1], (&b1)[E] = par[2];
+    // Next weight, post weight and bias, and scale, gate of the sample and 1 / (1 - p).
+    // Rows of 1,024 threads hold them in LDS, each thread its own (3,906 bf16 rows of 8,192
+    // with a gate per sample, a post and a next norm, forward and backward: 174 us, 282
+    // with all of them in registers, of which 68 a thread were spilled).
+    enum { kW2, kW1, kB1, kKs };
+    constexpr bool STAGED = TPR > 512 && HAS_Y;
+    __shared__ float staged[STAGED ? 4 : 1][STAGED ? E : 1][STAGED ? TPR : 1];
+    float par[4][E];
+    {
+        float w[3][E];
+        load_params<E, 3>({a.next.weight, HAS_Y ? a.post.weight : nullptr, HAS_Y ? a.post.bias : nullptr}, a.param, c,
+                          {1.f, 1.f, 0.f}, w);
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if constexpr (STAGED) staged[k][e][threadIdx.x] = w[k][e];
+                else par[k][e] = w[k][e];
+            }
+    }
+    auto param = [&](int k, int e) {
+        if constexpr (STAGED) return staged[k][e][threadIdx.x];
+        else return par[k][e];
+    };
     // Sums over this thread's rows: dw1, db1, dscale (1 - p), dw2, db2.
     float dw1[E], db1[E], dsc[E], dw2[E], db2[E];
 #pragma unroll
@@ -353,14 +373,15 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
         const Unit unit = unit_of(a, u);
         const int64_t gate_at = (int64_t)unit.sample * (a.gate_stride / (a.gate_dtype == P3D_F32 ? 4 : 2)) + c;
-        float ks[E], unit_acc[E];  // scale, gate of the sample and 1 / (1 - p); sum of gate keep b go
+        float unit_acc[E];  // sum of gate keep b go
         if constexpr (HAS_Y) {
-            float gs[E];
+            float gs[E], ks[E];
             load_param(a.scale, a.param, c, 1.f, ks);
             load_param(per_sample ? a.gate : nullptr, a.gate_dtype, gate_at, 1.f, gs);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                ks[e] *= gs[e] * mask.inv;
+                if constexpr (STAGED) staged[kKs][e][threadIdx.x] = ks[e] * gs[e] * mask.inv;
+                else par[kKs][e] = ks[e] * gs[e] * mask.inv;
                 unit_acc[e] = 0.f;
             }
         }
@@ -415,7 +436,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
                             xh1[e] = (xh1[e] - mean1) * rstd1;
-                            b[e] = xh1[e] * w1[e] + b1[e];
+                            b[e] = xh1[e] * param(kW1, e) + param(kB1, e);
                         }
                     } else {
 #pragma unroll
@@ -432,11 +453,11 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
                         float out = xh2[e];
-                        if constexpr (HAS_Y) out = a.alpha * out + ks[e] * (GATED ? g[e] * b[e] : b[e]);
+                        if constexpr (HAS_Y) out = a.alpha * out + param(kKs, e) * (GATED ? g[e] * b[e] : b[e]);
                         xh2[e] = (out - mean2) * rstd2;
                         dw2[e] += g2[e] * xh2[e];
                         db2[e] += g2[e];
-                        g2[e] *= w2[e];
+                        g2[e] *= param(kW2, e);
                         p[e] = g2[e] * xh2[e];
                     }
                     s[0] = layer2 ? at.own(g2) : 0.f;
@@ -462,11 +483,11 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
                         if constexpr (GATED) {
                             const float bg = b[e] * go[e];
                             unit_acc[e] += g[e] * bg;
-                            dg[e] = ks[e] * bg;
-                            db[e] = ks[e] * g[e] * go[e];
+                            dg[e] = param(kKs, e) * bg;
+                            db[e] = param(kKs, e) * g[e] * go[e];
                         } else {
                             unit_acc[e] += b[e] * go[e];
-                            db[e] = ks[e] * go[e];
+                            db[e] = param(kKs, e) * go[e];
                         }
                     }
                     if (mask.threshold) {
@@ -481,7 +502,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void k_block_bwd(BlockDev a) {
                         for (int e = 0; e < E; ++e) {
                             dw1[e] += db[e] * xh1[e];
                             db1[e] += db[e];
-                            db[e] *= w1[e];
+                            db[e] *= param(kW1, e);
                             p[e] = db[e] * xh1[e];
                         }
                         if (layer1) s[0] = at.own(db);
