@@ -141,7 +141,10 @@ std::pair<int64_t, int64_t> block_split(int64_t samples, int64_t tokens, int64_t
     const int64_t per_sample = (tokens + rows - 1) / rows, steps = per_sample * samples;
     int64_t wanted = round;
     if (!round && threads > 64) {
-        wanted = std::max<int64_t>(512, (1 << 18) / threads);
+        // Rows of 2 and 4 waves: several rounds, as below; of 8 and 16, whose workgroups fill
+        // a CU by two or one: one (fp32 over bf16, two norms, dropout, a gate per token: 1,000
+        // channels 106 us in 2,048 workgroups, 89 in 4,096; 6,144 channels 105 in 512, 99 in 256).
+        wanted = (threads <= 256 ? 1 << 19 : 1 << 18) / threads;
     } else if (!round) {
         // Several rounds, of at least four steps each once every CU has work: a workgroup
         // begins by loading the parameters (4,913 x 3 rows of 327: 21 us in 921, 25 in 3,685).
